@@ -207,6 +207,78 @@ rt_status rt_op_cross_entropy(rt_ctx* ctx, const float* logits_host, size_t rows
                               const float* weight, float* logp_host, int32_t* hits_out, int32_t* argmax_host,
                               float* dlogits_host);
 
+/* ------------------------------------------------------------------ row operations over the vocabulary
+ * Distillation from a teacher's top logits and the check of drafted tokens against a target's
+ * probabilities.  No counterpart in the reference, whose objectives are SFT and DPO (src/train.rs:269-297)
+ * and whose gate is greedy (src/eval.rs:152-221); the rows are those of its head (src/model.rs:561-609).
+ *
+ * A row holds the logits z of one position over the vocabulary.  With s_v = z_v / T - log sum_u exp(z_u / T)
+ * and p_v = exp(s_v) at a temperature T:
+ *   - a logit of -inf has probability 0; in a row of nothing else every p is 0 and every s is -inf;
+ *   - a row that holds a NaN or +inf has NaN for every p, s and loss, and for its gradient;
+ *   - among equal values (the two zeros are equal) the lowest index comes first.
+ * Rows are `ld` elements apart (ld >= vocab; what lies behind the vocabulary is neither read nor written),
+ * their elements RT_DT_F32, RT_DT_BF16 or RT_DT_F16; any element-aligned address is taken.  Sums are held in
+ * 32 bits within a thread and 64 beyond.  The device forms only launch on the ctx stream: they allocate
+ * nothing, share no workspace and may be captured; what a kernel finds wrong (an index out of range) is
+ * reported by the next rt_ctx_synchronize, like a wait that ran out.  The host forms take f32 rows. */
+#define RT_TOP_MAX 256      /* entries of a teacher's list, at most */
+#define RT_VOCAB_MAX 393216 /* elements of a row, at most */
+/* What becomes of the probability that a teacher's list leaves out: the list is normalised to one, or the rest is one
+ * more bucket against the student's rest. */
+enum { RT_DISTILL_RENORM = 0, RT_DISTILL_TAIL = 1 };
+
+/* The k largest logits of each row, largest first: their indices [rows x k], their s [rows x k], and (lse_dev, optional)
+ * log sum exp(z / T) [rows].  NaNs come before all other values.  1e-4 <= T <= 1e4. */
+rt_status rt_top_logits_dev(rt_ctx* ctx, const void* logits_dev, int dtype, size_t rows, size_t vocab, size_t ld,
+                            float temperature, int k, int32_t* index_dev, float* logp_dev, float* lse_dev);
+/* The divergence of each row from a teacher's list, and its gradient.  Entry j of a row's k: an index i_j (-1: no entry)
+ * and the teacher's log-probability t_j at it, as rt_top_logits_dev writes them.  An index that comes twice counts twice:
+ * the probabilities add up.
+ *   RENORM: q_j = exp(t_j) / sum exp(t);  loss = w sum q_j (log q_j - s_{i_j});  dz_v = (w / T) (p_v - q_v);
+ *           a row whose list has no mass gets 0 for both
+ *   TAIL:   q_j = exp(t_j), r = max(0, 1 - sum q), R = the student's mass outside the list;
+ *           loss = w (sum q_j (t_j - s_{i_j}) + r (log r - log R));
+ *           dz_v = (w / T) (p_v - q_v) inside the list, (w / T) p_v (1 - r / R) outside
+ * weight_dev [rows] (NULL: ones): a row of weight 0 is not read and gets zeros.  loss_dev [rows] may be NULL, and so may
+ * dlogits_dev ([rows x vocab], rows d_ld apart, of d_dtype; the logits' own place is allowed, any other overlap is not).
+ * row_scale_dev (optional, [rows]): the gradients are written without the factor w / T, which goes there: the form that
+ * rt_linear_backward_dev takes, in which f16 keeps its digits whatever the weights are. */
+rt_status rt_distill_dev(rt_ctx* ctx, const void* logits_dev, int dtype, size_t rows, size_t vocab, size_t ld,
+                         float temperature, const int32_t* index_dev, const float* teacher_logp_dev, int k, int mode,
+                         const float* weight_dev, float* loss_dev, void* dlogits_dev, int d_dtype, size_t d_ld,
+                         float* row_scale_dev);
+/* p of each row, as prob_dtype; the logits' own place is allowed, any other overlap is not. */
+rt_status rt_softmax_dev(rt_ctx* ctx, const void* logits_dev, int dtype, size_t rows, size_t vocab, size_t ld,
+                         float temperature, void* prob_dev, int prob_dtype, size_t prob_ld);
+/* Which drafted tokens stand against the target's probabilities.  Sequence s drafted the tokens
+ * draft_tok[draft_offsets[s] .. draft_offsets[s+1]) (n_draft in all; none is allowed); target row draft_offsets[s] + s + i
+ * holds the target's probabilities at its draft i, and the row behind its last draft's those that follow them all
+ * (n_draft + n_seq rows); draft row draft_offsets[s] + i the probabilities that draft i was drawn from (draft_prob_dev NULL:
+ * the drafts were certain, q = 1).  With u = u_accept[draft] in [0, 1), a draft d stands if all before it stand and
+ * u q(d) < p(d).  accepted[s] is how many do.  token[s] follows them: drawn with u_sample[s] in [0, 1) from
+ * max(p - q, 0) at the first draft that does not stand (p without d, for certain drafts; p where nothing is left), or from
+ * p of the last row: the lowest index at which the running sum exceeds u_sample times the whole sum.  Products and sums are
+ * in 64 bits, so that 16-bit and 32-bit probabilities are compared exactly.  What is no finite positive number counts as
+ * no mass; a row without mass gives token -1; a number u_sample that is not below 1 gives the last index with mass.  A token
+ * outside the vocabulary or offsets that do not ascend from 0 to n_draft are RT_ERR_BAD_INDEX (their sequence: accepted 0,
+ * token -1). */
+rt_status rt_verify_draft_dev(rt_ctx* ctx, const void* target_prob_dev, size_t target_ld, const void* draft_prob_dev,
+                              size_t draft_ld, int dtype, size_t vocab, const int32_t* draft_tok_dev,
+                              const int32_t* draft_offsets_dev, size_t n_seq, size_t n_draft, const float* u_accept_dev,
+                              const float* u_sample_dev, int32_t* accepted_dev, int32_t* token_dev);
+/* The same operations with host buffers, rows of `vocab` floats. */
+rt_status rt_op_top_logits(rt_ctx* ctx, const float* logits_host, size_t rows, size_t vocab, float temperature, int k,
+                           int32_t* index_host, float* logp_host, float* lse_host);
+rt_status rt_op_distill(rt_ctx* ctx, const float* logits_host, size_t rows, size_t vocab, float temperature,
+                        const int32_t* index_host, const float* teacher_logp_host, int k, int mode, const float* weight_host,
+                        float* loss_host, float* dlogits_host);
+rt_status rt_op_softmax(rt_ctx* ctx, const float* logits_host, size_t rows, size_t vocab, float temperature, float* prob_host);
+rt_status rt_op_verify_draft(rt_ctx* ctx, const float* target_prob_host, const float* draft_prob_host, size_t vocab,
+                             const int32_t* draft_tok_host, const int32_t* draft_offsets_host, size_t n_seq,
+                             const float* u_accept_host, const float* u_sample_host, int32_t* accepted_host,
+                             int32_t* token_host);
+
 /* ------------------------------------------------------------------ level 2: struct Linear / struct Lora
  * src/linear.rs:9-122.  y = W.x + b + (alpha/r).B.A.x forward; dx = W^T.dy + (LoRA term) and
  * the adapter gradients dA, dB backward.  Device-resident: this is the performance boundary,

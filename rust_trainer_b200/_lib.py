@@ -140,6 +140,14 @@ def _declare(L: C.CDLL) -> None:
         "rt_op_swiglu": (i32, [vp, f32p, f32p, sz, sz, f32p]),
         "rt_op_swiglu_backward": (i32, [vp, f32p, f32p, f32p, sz, sz, f32p, f32p]),
         "rt_op_cross_entropy": (i32, [vp, f32p, sz, sz, i32p, f32p, f32p, i32p, i32p, f32p]),
+        "rt_top_logits_dev": (i32, [vp, vp, ci, sz, sz, sz, cf, ci, vp, vp, vp]),
+        "rt_distill_dev": (i32, [vp, vp, ci, sz, sz, sz, cf, vp, vp, ci, ci, vp, vp, vp, ci, sz, vp]),
+        "rt_softmax_dev": (i32, [vp, vp, ci, sz, sz, sz, cf, vp, ci, sz]),
+        "rt_verify_draft_dev": (i32, [vp, vp, sz, vp, sz, ci, sz, vp, vp, sz, sz, vp, vp, vp, vp]),
+        "rt_op_top_logits": (i32, [vp, f32p, sz, sz, cf, ci, i32p, f32p, f32p]),
+        "rt_op_distill": (i32, [vp, f32p, sz, sz, cf, i32p, f32p, ci, ci, f32p, f32p, f32p]),
+        "rt_op_softmax": (i32, [vp, f32p, sz, sz, cf, f32p]),
+        "rt_op_verify_draft": (i32, [vp, f32p, f32p, sz, i32p, i32p, sz, f32p, f32p, i32p, i32p]),
     })
     for name, (res, args) in sig.items():
         fn = getattr(L, name)

@@ -140,3 +140,68 @@ def cross_entropy(ctx: Context, logits, target, weight=None, want_argmax=False, 
     if dl is not None:
         out["dlogits"] = dl
     return out
+
+
+#: what becomes of the probability that a teacher's list leaves out (RT_DISTILL_*)
+DISTILL_MODES = {"renorm": 0, "tail": 1}
+
+
+def distill_mode(mode: str) -> int:
+    if mode not in DISTILL_MODES:
+        raise RtError(7, f"unknown distillation mode {mode!r}")
+    return DISTILL_MODES[mode]
+
+
+def _rows(a, what: str):
+    a = _f(a)
+    if a.ndim != 2:
+        raise RtError(1, f"{what}: rows expected")
+    return a
+
+
+def top_logits(ctx: Context, logits, k: int, temperature: float = 1.0):
+    """The k largest logits of each row (ties: the lowest index first): (index [rows x k], log-probability [rows x k],
+    log-sum-exp [rows]) at the temperature.  No counterpart in the reference."""
+    z = _rows(logits, "top_logits")
+    rows = z.shape[0]
+    index, logp, lse = np.empty((rows, max(k, 0)), np.int32), np.empty((rows, max(k, 0)), np.float32), np.empty(rows, np.float32)
+    ctx.check(lib().rt_op_top_logits(ctx._h, _fp(z), rows, z.shape[1], temperature, k, _ip(index), _fp(logp), _fp(lse)))
+    return index, logp, lse
+
+
+def distill(ctx: Context, logits, index, teacher_logp, weight=None, temperature: float = 1.0, mode: str = "renorm", want_dlogits: bool = False):
+    """Divergence of each row from a teacher's list (index -1: no entry) and its gradient; dict(loss[, dlogits]).  The teacher's
+    probabilities are normalised over the list ("renorm"), or what they leave is one more bucket ("tail")."""
+    z, index, t = _rows(logits, "distill"), _i(index), _f(teacher_logp)
+    rows = z.shape[0]
+    w = None if weight is None else _f(weight)
+    if index.ndim != 2 or index.shape[0] != rows or t.shape != index.shape or (w is not None and w.shape != (rows,)):
+        raise RtError(1, "distill: the lists and weights do not fit the rows")
+    loss = np.empty(rows, np.float32)
+    d = np.empty_like(z) if want_dlogits else None
+    ctx.check(lib().rt_op_distill(ctx._h, _fp(z), rows, z.shape[1], temperature, _ip(index), _fp(t), index.shape[1], distill_mode(mode),
+                                  None if w is None else _fp(w), _fp(loss), None if d is None else _fp(d)))
+    return dict(loss=loss) if d is None else dict(loss=loss, dlogits=d)
+
+
+def softmax(ctx: Context, logits, temperature: float = 1.0) -> np.ndarray:
+    """Probabilities of each row at the temperature."""
+    z = _rows(logits, "softmax")
+    p = np.empty_like(z)
+    ctx.check(lib().rt_op_softmax(ctx._h, _fp(z), z.shape[0], z.shape[1], temperature, _fp(p)))
+    return p
+
+
+def verify_draft(ctx: Context, target_prob, draft_prob, draft_tok, offsets, u_accept, u_sample):
+    """Which drafted tokens stand and the token that follows them: (accepted [n_seq], token [n_seq]).  Sequence s drafted
+    draft_tok[offsets[s]:offsets[s + 1]]; its rows of target_prob are its drafts' and one behind them; draft_prob None: the drafts
+    were certain.  u_accept has a number in [0, 1) per draft, u_sample one per sequence."""
+    p, tok, off, ua, us = _rows(target_prob, "verify_draft"), _i(draft_tok), _i(offsets), _f(u_accept), _f(u_sample)
+    q = None if draft_prob is None else _rows(draft_prob, "verify_draft")
+    n_seq, n = us.size, tok.size
+    if off.shape != (n_seq + 1,) or off[-1] != n or ua.size != n or p.shape[0] != n + n_seq or (q is not None and q.shape != (n, p.shape[1])):
+        raise RtError(1, "verify_draft: drafts, rows and random numbers do not fit each other")
+    accepted, token = np.empty(n_seq, np.int32), np.empty(n_seq, np.int32)
+    ctx.check(lib().rt_op_verify_draft(ctx._h, _fp(p), None if q is None else _fp(q), p.shape[1], _ip(tok), _ip(off), n_seq, _fp(ua), _fp(us),
+                                       _ip(accepted), _ip(token)))
+    return accepted, token
