@@ -216,6 +216,7 @@ rt_status rt_op_cross_entropy(rt_ctx* ctx, const float* logits_host, size_t rows
  * and p_v = exp(s_v) at a temperature T:
  *   - a logit of -inf has probability 0; in a row of nothing else every p is 0 and every s is -inf;
  *   - a row that holds a NaN or +inf has NaN for every p, s and loss, and for its gradient;
+ *   - a probability below 2^-126 of the row's largest may come out as 0;
  *   - among equal values (the two zeros are equal) the lowest index comes first.
  * Rows are `ld` elements apart (ld >= vocab; what lies behind the vocabulary is neither read nor written),
  * their elements RT_DT_F32, RT_DT_BF16 or RT_DT_F16; any element-aligned address is taken.  Sums are held in
