@@ -5,10 +5,13 @@
 // Only where they are too many (values that tie, masked rows) is a bound sought that leaves fewer, by bisection over values and
 // indices.
 #include "vocab_rows.cuh"
+#include <algorithm>
 
 namespace rt {
 
 constexpr int TOP_ROOM = 2048;  // candidates
+// slots of the row's region at least: it takes the candidates once more when the row is no longer needed
+constexpr int TOP_LEAST_SLOTS = TOP_ROOM / 2 + 1;
 static_assert(TOP_ROOM / VR_MAX_CLUSTER >= RT_TOP_MAX, "k elements of one CTA's share have to fit");
 // An element as an integer, all different: its value's order above, the lower index in front.
 constexpr int TOP_INDEX_BITS = 19;
@@ -19,8 +22,7 @@ __device__ __forceinline__ TopKey top_key(float v, int c) {
 }
 
 struct TopStat {
-  double s;
-  float m;
+  float m, s;
   uint32_t each, own;  // what every warp of the cluster, and every warp of this CTA, has to have for k elements
 };
 
@@ -40,20 +42,22 @@ __device__ __forceinline__ uint32_t warp_sort(uint32_t v) {
 }
 
 template <class T>
-__global__ void __launch_bounds__(VR_THREADS, 2) top_logits_kernel(const T* z, size_t ld, int vocab, float t, ExpT ex, int k, int* index, float* logp, float* lse) {
+__global__ void __launch_bounds__(VR_THREADS, 2) top_logits_kernel(const T* z, size_t ld, int vocab, float t, ExpT ex, int k, int* index, float* logp, float* lse, int* status) {
   constexpr int VEC = RowPart<T>::VEC, STEP = RowPart<T>::STEP;
   extern __shared__ uint4 slots[];
+  __shared__ uint64_t bars[VR_MAX_STEPS];
   __shared__ TopStat stat[VR_MAX_CLUSTER * VR_WARPS];
   __shared__ int s_n, s_count[2], counts[2][VR_MAX_CLUSTER];
   __shared__ double s_log_sum;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   cluster_arrive_relaxed();
   const size_t r = cluster_id();
-  const RowPart<T> part(z + r * ld, vocab, slots);
+  const RowPart<T> part(z + r * ld, vocab, slots, bars, status);
   part.load();
-  TopKey* room = (TopKey*)(slots + part.n_it_most() * VR_THREADS);
+  TopKey* room = (TopKey*)(slots + max(part.n_it_most() * VR_THREADS, TOP_LEAST_SLOTS));
   const int room_each = TOP_ROOM / part.size;
   if (tid == 0) s_n = s_count[0] = s_count[1] = 0;
+  __syncthreads();
   MaxSum ms;
   for (int s = 0; s < part.n_steps; ++s) {
     float x[16];
@@ -66,17 +70,16 @@ __global__ void __launch_bounds__(VR_THREADS, 2) top_logits_kernel(const T* z, s
   TopStat st;
   st.each = __shfl_sync(0xffffffffu, sorted, (k + warps - 1) / warps - 1);
   st.own = __shfl_sync(0xffffffffu, sorted, (k + VR_WARPS - 1) / VR_WARPS - 1);
-  st.s = warp_join(ms.m, ms.s, ex, &st.m);
+  st.s = warp_join(ms, ex, &st.m);
   cluster_wait();  // the other CTAs run: their shared memory may be written
   if (lane < part.size) {
     const uint32_t to = mapa_u32(smem_u32(&stat[part.rank * VR_WARPS + warp]), lane);
-    st_cluster(to, st.s);
-    st_cluster(to + 8, __float_as_uint(st.m), st.each);
-    st_cluster(to + 16, (int)st.own);
+    st_cluster(to, __float_as_uint(st.m), __float_as_uint(st.s));
+    st_cluster(to + 8, st.each, st.own);
   }
   cluster_arrive();
   cluster_wait();
-  const TopStat none{0.0, -INFINITY, 0xffffffffu, 0xffffffffu}, a = lane < warps ? stat[lane] : none, b = lane + 32 < warps ? stat[lane + 32] : none;
+  const TopStat none{-INFINITY, 0.0f, 0xffffffffu, 0xffffffffu}, a = lane < warps ? stat[lane] : none, b = lane + 32 < warps ? stat[lane + 32] : none;
   uint32_t own = a.own, own_b = b.own;  // eight neighbours are a CTA's warps
 #pragma unroll
   for (int o = 1; o < VR_WARPS; o *= 2) {
@@ -86,27 +89,23 @@ __global__ void __launch_bounds__(VR_THREADS, 2) top_logits_kernel(const T* z, s
   const uint32_t own_max = __reduce_max_sync(0xffffffffu, max(lane < warps ? own : 0u, lane + 32 < warps ? own_b : 0u));
   const uint32_t bound = max(__reduce_min_sync(0xffffffffu, min(a.each, b.each)), own_max);
   float m;
-  const float ab = max_nan(a.m, b.m);
-  double sum = ab > -INFINITY ? a.s * (double)ex(a.m - ab) + b.s * (double)ex(b.m - ab) : 0.0;
-  sum = warp_join(ab, sum, ex, &m);
+  const double sum = cluster_join(a.m, a.s, b.m, b.s, ex, &m);
 
   const uint32_t leader_room = mapa_u32(smem_u32(room), 0);
   auto push = [&](TopKey key) {
     const int p = atomicAdd(&s_n, 1);
     if (p < room_each) st_cluster(leader_room + (uint32_t)(part.rank * room_each + p) * 8, key);
   };
-  // a warp takes the vectors of its threads that reach the bound one thread after the other, a vector a lane
-  for (unsigned with = __ballot_sync(0xffffffffu, my_top >= bound); with; with &= with - 1) {
-    const int owner = warp * 32 + __ffs(with) - 1;
-    for (int it = lane; it < part.n_it; it += 32) {
-      if (part.column(it, owner) >= vocab) continue;
+  if (my_top >= bound) {  // a few threads of a warp, which look for their elements side by side
+    const float from = order32_value(bound);
+    for (int it = 0; it < part.n_it; ++it) {
+      const int c0 = part.column(it, tid);
+      if (c0 >= vocab) break;
       float x[VEC];
-      RowPart<T>::unpack(slots[it * VR_THREADS + owner], x);
+      RowPart<T>::unpack(slots[it * VR_THREADS + tid], x);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        const int c = part.column(it, owner) + i;
-        if (order32(x[i]) >= bound && c >= 0 && c < vocab) push(top_key(x[i], c));
-      }
+      for (int i = 0; i < VEC; ++i)
+        if (!(x[i] < from) && c0 + i >= 0 && c0 + i < vocab) push(top_key(x[i], c0 + i));  // NaN too
     }
   }
   // every CTA learns how many each has: `to` is written in all of them
@@ -180,25 +179,50 @@ __global__ void __launch_bounds__(VR_THREADS, 2) top_logits_kernel(const T* z, s
     if (lse) lse[r] = bad ? NAN : (float)((double)m / t + s_log_sum);
   }
   __syncthreads();
-  for (int l = 0; l < part.size; ++l)
-    for (int i = tid; i < counts[0][l]; i += VR_THREADS) {
+  // The lists one behind the other in what held the row: orders, filled up with the lowest to a multiple of four, and columns.
+  int n = 0;
+  for (int l = 0; l < part.size; ++l) n += counts[0][l];
+  const int n4 = (n + 3) / 4;
+  uint32_t *order = (uint32_t*)slots, *column = order + 4 * n4;
+  int before = 0;
+  for (int l = 0; l < part.size; ++l) {
+    const int here = counts[0][l];
+    for (int i = tid; i < here; i += VR_THREADS) {
       const TopKey key = room[l * room_each + i];
-      int rank = 0;
-      for (int o = 0; o < part.size; ++o)
-        for (int j = 0; j < counts[0][o]; ++j) rank += room[o * room_each + j] > key;
-      if (rank >= k) continue;
-      const float v = order32_value((uint32_t)(key >> TOP_INDEX_BITS));
-      index[r * k + rank] = (1 << TOP_INDEX_BITS) - 1 - (int)(key & ((1 << TOP_INDEX_BITS) - 1));
-      logp[r * k + rank] = bad ? NAN : v == -INFINITY ? -INFINITY : (float)(((double)v - m) / t - s_log_sum);
+      order[before + i] = (uint32_t)(key >> TOP_INDEX_BITS);
+      column[before + i] = (1 << TOP_INDEX_BITS) - 1 - (uint32_t)(key & ((1 << TOP_INDEX_BITS) - 1));
     }
+    before += here;
+  }
+  if (tid < 4 * n4 - n) order[n + tid] = 0;
+  __syncthreads();
+  const double log_sum = s_log_sum;
+  for (int i = tid; i < n; i += VR_THREADS) {
+    const uint32_t mine = order[i];
+    int rank = 0, same = -1;
+#pragma unroll 4
+    for (int j = 0; j < n4; ++j) {
+      const uint4 o = ((const uint4*)order)[j];
+      rank += (o.x > mine) + (o.y > mine) + (o.z > mine) + (o.w > mine);
+      same += (o.x == mine) + (o.y == mine) + (o.z == mine) + (o.w == mine);
+    }
+    if (rank >= k) continue;
+    if (same > 0)
+      for (int j = 0; j < n; ++j) rank += order[j] == mine && column[j] < column[i];
+    if (rank >= k) continue;
+    const float v = order32_value(mine);
+    index[r * k + rank] = (int)column[i];
+    logp[r * k + rank] = bad ? NAN : v == -INFINITY ? -INFINITY : (float)(((double)v - m) / t - log_sum);
+  }
 }
 
 int launch_top_logits(rt_ctx* c, const VocabRows& z, size_t rows, int vocab, float temperature, int k, int* index, float* logp, float* lse) {
   const RowShape shape = row_shape(vocab, z.dtype);
+  const size_t smem = std::max(shape.slots, (size_t)TOP_LEAST_SLOTS) * 16 + TOP_ROOM * 8;
   return with_dtype(z.dtype, [&](auto* zt) {
     using T = std::remove_pointer_t<decltype(zt)>;
-    return launch_clusters(c, top_logits_kernel<T>, rows, shape.cluster, shape.slots * 16 + TOP_ROOM * 8, (const T*)z.p, z.ld, vocab, temperature,
-                           exp_t(temperature), k, index, logp, lse);
+    return launch_clusters(c, top_logits_kernel<T>, rows, shape.cluster, smem, (const T*)z.p, z.ld, vocab, temperature,
+                           exp_t(temperature), k, index, logp, lse, c->status_dev);
   });
 }
 

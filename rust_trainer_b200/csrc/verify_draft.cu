@@ -7,7 +7,19 @@ namespace rt {
 
 constexpr int VD_EIGHTHS = 8;
 
-__device__ __forceinline__ double mass_of(double v) { return v > 0.0 && v < (double)INFINITY ? v : 0.0; }
+__device__ __forceinline__ bool is_mass(float v) { return v > 0.0f && v < INFINITY; }
+
+// A sum as two floats: the second holds what the first rounds away (Knuth's two-sum), so that sums of many elements are exact to some
+// 2^-45, at a fraction of the conversions and additions in 64 bits, which took ten times as long here.
+struct Sum2 {
+  float hi = 0.0f, lo = 0.0f;
+  __device__ __forceinline__ void add(float v, float v_lo) {
+    const float s = hi + v, b = s - hi;
+    lo += (hi - (s - b)) + (v - b) + v_lo;
+    hi = s;
+  }
+  __device__ __forceinline__ double value() const { return (double)hi + (double)lo; }
+};
 
 // The mass that a row leaves: max(p - q, 0), or p, or p without an index.  Vectors of 16 aligned bytes of p's row.
 template <class T>
@@ -22,26 +34,39 @@ struct Left {
     n_vec = (phase + vocab + VEC - 1) / VEC;
   }
   __device__ __forceinline__ int column(int v) const { return v * VEC - phase; }
-  __device__ __forceinline__ void get(int v, double (&x)[VEC]) const {
+  // 16 bytes of p and of q (0 where there are none)
+  __device__ __forceinline__ void load(int v, uint4* a, uint4* b) const {
     const int c = column(v);
-    float a[VEC], b[VEC];
+    *a = *b = make_uint4(0, 0, 0, 0);
+    if (v >= n_vec) return;
     if (c >= 0 && c + VEC <= vocab) {
-      RowPart<T>::unpack(__ldg((const uint4*)(p + c)), a);
-      if (q && same_phase) RowPart<T>::unpack(__ldg((const uint4*)(q + c)), b);
+      *a = __ldg((const uint4*)(p + c));
+      if (q && same_phase) *b = __ldg((const uint4*)(q + c));
       else if (q) {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) b[i] = to_f32(q[c + i]);
+        for (int i = 0; i < VEC; ++i) ((T*)b)[i] = q[c + i];
       }
     } else {
-#pragma unroll
       for (int i = 0; i < VEC; ++i) {
-        const bool in = c + i >= 0 && c + i < vocab;
-        a[i] = in ? to_f32(p[c + i]) : 0.0f;
-        b[i] = in && q ? to_f32(q[c + i]) : 0.0f;
+        if (c + i < 0 || c + i >= vocab) continue;
+        ((T*)a)[i] = p[c + i];
+        if (q) ((T*)b)[i] = q[c + i];
       }
     }
+  }
+  // the masses as sums of two floats: a difference of two floats is one rounded and what the rounding lost
+  __device__ __forceinline__ void masses(int v, const uint4& a, const uint4& b, float (&x)[VEC], float (&lo)[VEC]) const {
+    float pa[VEC], pb[VEC];
+    RowPart<T>::unpack(a, pa);
+    RowPart<T>::unpack(b, pb);
+    const int skip = without - column(v);
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) x[i] = c + i == without ? 0.0 : mass_of(q ? (double)a[i] - (double)b[i] : (double)a[i]);
+    for (int i = 0; i < VEC; ++i) {
+      const float d = pa[i] - pb[i], bb = d - pa[i], e = (pa[i] - (d - bb)) - (pb[i] + bb);
+      const bool on = is_mass(d) && i != skip;
+      x[i] = on ? d : 0.0f;
+      lo[i] = on ? e : 0.0f;
+    }
   }
 };
 
@@ -85,76 +110,86 @@ __global__ void __launch_bounds__(VR_THREADS) verify_draft_kernel(const T* P, si
   Left<T> left(p_row, Q && at < e ? Q + (size_t)at * ld_q : nullptr, !Q && at < e ? tok[at] : -1, vocab);
   // vectors of an eighth of a piece, in rounds of a warp
   const int rounds = (left.n_vec + 32 * VD_EIGHTHS * pieces - 1) / (32 * VD_EIGHTHS * pieces), eighth = rounds * 32, lo = piece * eighth * VD_EIGHTHS;
-  double sums[VD_EIGHTHS], total = 0.0, before = 0.0, mine = 0.0;
-  const double* masses = nullptr;
-  for (int pass = 0; pass < 2; ++pass) {
-#pragma unroll
-    for (int j = 0; j < VD_EIGHTHS; ++j) sums[j] = 0.0;
+  double sums[VD_EIGHTHS], total = 0.0, run = 0.0, want = 0.0;
+  int chosen = -1;  // the piece that holds the token
+  for (int pass = 0; pass < 2 && chosen < 0; ++pass) {
+    if (pass > 0) left = Left<T>(p_row, nullptr, -1, vocab);  // nothing was left: the target's own probabilities
+    Sum2 acc[VD_EIGHTHS];
     for (int t = 0; t < rounds; ++t) {
 #pragma unroll
-      for (int j = 0; j < VD_EIGHTHS; ++j) {
-        const int v = lo + j * eighth + t * 32 + lane;
-        if (v >= left.n_vec) continue;
-        double x[VEC];
-        left.get(v, x);
+      for (int j0 = 0; j0 < VD_EIGHTHS; j0 += 4) {
+        uint4 pa[4], qa[4];
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) sums[j] += x[i];
+        for (int j = 0; j < 4; ++j) left.load(lo + (j0 + j) * eighth + t * 32 + lane, pa + j, qa + j);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float x[VEC], x_lo[VEC];
+          left.masses(lo + (j0 + j) * eighth + t * 32 + lane, pa[j], qa[j], x, x_lo);
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) acc[j0 + j].add(x[i], x_lo[i]);
+        }
       }
     }
+    double mine = 0.0;
 #pragma unroll
-    for (int j = 0; j < VD_EIGHTHS; ++j) sums[j] = warp_sum_f64(sums[j]);
-    mine = 0.0;
+    for (int j = 0; j < VD_EIGHTHS; ++j) sums[j] = warp_sum_f64(acc[j].value());
 #pragma unroll
     for (int j = 0; j < VD_EIGHTHS; ++j) mine += sums[j];
     if (lane < size) st_cluster(mapa_u32(smem_u32(&mass[pass][piece]), lane), mine);
     cluster_arrive();
     cluster_wait();
-    total = before = 0.0;
-    masses = mass[pass];
-    for (int i = 0; i < pieces; ++i) {
-      if (i == piece) before = total;
-      total += masses[i];
+    // Running sums over the pieces, two a lane, the same in every warp.  The token's piece is the first with mass whose sum exceeds
+    // `want`, or the last with mass where none does.
+    const double m0 = 2 * lane < pieces ? mass[pass][2 * lane] : 0.0, m1 = 2 * lane + 1 < pieces ? mass[pass][2 * lane + 1] : 0.0;
+    double up = m0 + m1;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+      const double y = __shfl_up_sync(0xffffffffu, up, o);
+      if (lane >= o) up += y;
     }
-    if (total > 0.0) break;
-    left = Left<T>(p_row, nullptr, -1, vocab);  // nothing is left: the target's own probabilities
+    total = __shfl_sync(0xffffffffu, up, 31);
+    if (!(total > 0.0)) continue;
+    want = u < 0.0f ? 0.0 : (double)u * total;
+    double in_front = __shfl_up_sync(0xffffffffu, up, 1);  // of the lane's two pieces
+    if (lane == 0) in_front = 0.0;
+    const unsigned over0 = __ballot_sync(0xffffffffu, m0 > 0.0 && in_front + m0 > want), over1 = __ballot_sync(0xffffffffu, m1 > 0.0 && up > want);
+    const unsigned with0 = __ballot_sync(0xffffffffu, m0 > 0.0), with1 = __ballot_sync(0xffffffffu, m1 > 0.0);
+    if (over0 | over1) {
+      const int l = __ffs(over0 | over1) - 1;
+      chosen = 2 * l + !(over0 >> l & 1);
+    } else {
+      const int l = 31 - __clz(with0 | with1);
+      chosen = 2 * l + (with1 >> l & 1);
+    }
+    run = __shfl_sync(0xffffffffu, in_front, chosen / 2);
+    const double m_even = __shfl_sync(0xffffffffu, m0, chosen / 2);
+    if (chosen & 1) run += m_even;
   }
-  if (!(total > 0.0)) {
-    if (tid == 0 && rank == 0) token[s] = -1;
-    return;
-  }
-  // The piece whose running sum is the first to exceed `want`; the last one with mass where none does.
-  const double want = u < 0.0f ? 0.0 : (double)u * total;
-  const bool none = !(total > want);
-  bool here = mine > 0.0 && !(before > want) && before + mine > want;
-  if (none) {
-    here = mine > 0.0;
-    for (int i = piece + 1; i < pieces; ++i) here &= !(masses[i] > 0.0);
-  }
-  if (!here) return;
-  double run = before;
+  if (chosen < 0 && tid == 0 && rank == 0) token[s] = -1;
+  if (chosen != piece) return;
+  // the eighth and the vector and the element, by the same rule
   int first = -1, last = -1;
+  double run_last = run;
 #pragma unroll
-  for (int j = 0; j < VD_EIGHTHS; ++j) {  // the eighth, by the same rule
-    if (sums[j] > 0.0) {
+  for (int j = 0; j < VD_EIGHTHS; ++j) {
+    if (first < 0 && sums[j] > 0.0) {
       last = j;
-      if (first < 0 && run + sums[j] > want) first = j;
-      else if (first < 0) run += sums[j];
+      run_last = run;
+      if (run + sums[j] > want) first = j;
+      else run += sums[j];
     }
   }
-  if (first < 0) {
-    first = last;
-    run = before;
-#pragma unroll
-    for (int j = 0; j < VD_EIGHTHS; ++j)
-      if (j < last) run += sums[j];
-  }
+  run = run_last;
   int found = -1, at_last = -1;
   for (int t = 0; t < rounds && found < 0; ++t) {
-    const int v = lo + first * eighth + t * 32 + lane;
-    double x[VEC] = {}, sum = 0.0;
-    if (v < left.n_vec) left.get(v, x);
+    const int v = lo + last * eighth + t * 32 + lane;
+    uint4 pa, qa;
+    float x[VEC], x_lo[VEC];
+    left.load(v, &pa, &qa);
+    left.masses(v, pa, qa, x, x_lo);
+    double sum = 0.0;
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) sum += x[i];
+    for (int i = 0; i < VEC; ++i) sum += (double)x[i] + (double)x_lo[i];
     double up = sum;  // with the lanes in front
 #pragma unroll
     for (int o = 1; o < 32; o *= 2) {
@@ -166,8 +201,8 @@ __global__ void __launch_bounds__(VR_THREADS) verify_draft_kernel(const T* P, si
     double part = run + (up - sum);
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
-      part += x[i];
-      if (x[i] > 0.0) {
+      part += (double)x[i] + (double)x_lo[i];
+      if (x[i] > 0.0f) {
         end = left.column(v) + i;
         if (hit < 0 && part > want) hit = end;
       }

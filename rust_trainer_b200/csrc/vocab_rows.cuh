@@ -68,10 +68,12 @@ __device__ __forceinline__ float order32_value(uint32_t o) {
 // ---- a row in the shared memory of a cluster
 // A row is cut into vectors of 16 aligned bytes (the first and the last may stick out of it: what is outside reads as -inf), these into
 // blocks of VR_THREADS, and the blocks are dealt to the cluster's CTAs in turn, so that each sees a sample of the whole row
-// wherever its large values lie.  A thread reads in shared memory only what it copied there itself, so that no barrier stands between
-// the copies and their use; all of them are in flight at once.
+// wherever its large values lie.  A CTA's blocks are bulk copies, all of them in flight at once; those of a step, 16 elements a
+// thread, complete one barrier.
 constexpr uint32_t VR_MOST_SMEM = 214 * 1024;  // dynamic shared memory: RT_VOCAB_MAX elements of 32 bits on eight CTAs, and what is beside them
 constexpr int VR_THREADS = 256, VR_WARPS = VR_THREADS / 32, VR_MAX_CLUSTER = 8;
+constexpr int VR_MAX_STEPS = 16;  // 13 are the most: RT_VOCAB_MAX elements, 16 a thread and step
+constexpr int SITE_VOCAB_ROW = 701;
 
 __device__ __forceinline__ size_t cluster_id() {
   uint32_t r;
@@ -98,14 +100,18 @@ __device__ __forceinline__ void st_cluster(uint32_t addr, unsigned long long v) 
 __device__ __forceinline__ void st_cluster(uint32_t addr, int v) {
   asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
 }
-// wait until at most n of the thread's copy groups are under way (or fewer, where n is large)
-__device__ __forceinline__ void cp_async_wait_n(int n) {
-  if (n <= 0) cp_async_wait<0>();
-  else if (n == 1) cp_async_wait<1>();
-  else if (n == 2) cp_async_wait<2>();
-  else if (n == 3) cp_async_wait<3>();
-  else if (n <= 5) cp_async_wait<4>();
-  else cp_async_wait<6>();
+// The matmul's wait gives up when another kernel has reported anything; here an index out of range in one row must not end the
+// others' waits, so that only the time limit does.
+static __device__ __noinline__ void row_wait_slow(uint64_t* bar, int* status) {
+  const long long t0 = clock64();
+  for (;;) {
+    for (int i = 0; i < 256; ++i)
+      if (mbar_try_wait(bar, 0)) return;
+    if (clock64() - t0 > MBAR_WAIT_LIMIT_CYCLES) {
+      report_status(status, SITE_VOCAB_ROW);
+      return;
+    }
+  }
 }
 
 template <class T>
@@ -115,9 +121,11 @@ struct RowPart {
   const T* row;
   int phase, vocab, rank, size, n_vec, n_it, n_steps;  // n_it: vectors per thread of this CTA at most
   uint4* slots;                                        // [n_it][VR_THREADS]
+  uint64_t* bars;                                      // [VR_MAX_STEPS]
+  int* status;
 
-  __device__ __forceinline__ RowPart(const T* row_, int vocab_, uint4* slots_)
-      : row(row_), vocab(vocab_), rank((int)cluster_ctarank()), size((int)cluster_size()), slots(slots_) {
+  __device__ __forceinline__ RowPart(const T* row_, int vocab_, uint4* slots_, uint64_t* bars_, int* status_)
+      : row(row_), vocab(vocab_), rank((int)cluster_ctarank()), size((int)cluster_size()), slots(slots_), bars(bars_), status(status_) {
     phase = (int)(((uintptr_t)row & 15) / sizeof(T));
     n_vec = (phase + vocab + VEC - 1) / VEC;
     const int blocks = (n_vec + VR_THREADS - 1) / VR_THREADS;
@@ -126,46 +134,70 @@ struct RowPart {
   }
   // slots per thread of the cluster's first CTA, which has most: where what lies behind them starts in every CTA
   __device__ __forceinline__ int n_it_most() const { return ((n_vec + VR_THREADS - 1) / VR_THREADS + size - 1) / size; }
-  // the vector that a thread's `it`-th slot holds, and the column of its first element
-  __device__ __forceinline__ int vector(int it) const { return (it * size + rank) * VR_THREADS + (int)threadIdx.x; }
-  __device__ __forceinline__ int column(int it, int thread) const { return ((it * size + rank) * VR_THREADS + thread) * VEC - phase; }
+  __device__ __forceinline__ int first_vector(int it) const { return (it * size + rank) * VR_THREADS; }
+  // the column of a slot's first element
+  __device__ __forceinline__ int column(int it, int thread) const { return (first_vector(it) + thread) * VEC - phase; }
   // where column `c` lies: its CTA, and the index of its vector's slot there
-  __device__ __forceinline__ int owner(int c, int* slot, int* lane) const {
+  __device__ __forceinline__ int owner(int c, int* slot, int* elem) const {
     const int v = (c + phase) / VEC, block = v / VR_THREADS;
     *slot = block / size * VR_THREADS + v % VR_THREADS;
-    *lane = (c + phase) % VEC;
+    *elem = (c + phase) % VEC;
     return block % size;
   }
+  // Starts the copies; a __syncthreads() has to follow before the first get().
   __device__ __forceinline__ void load() const {
-    for (int s = 0; s < n_steps; ++s) {
+    const int tid = threadIdx.x;
+    if (tid < 32) {
+      if (tid < n_steps) mbar_init(bars + tid, 1);
+      mbar_fence_init();
+      fence_proxy_async_smem();
+      __syncwarp();
+      const int first_whole = phase ? 1 : 0, end_whole = (phase + vocab) / VEC;  // vectors that lie in the row
+      if (tid < n_steps) {
+        uint32_t bytes = 0;
 #pragma unroll
-      for (int j = 0; j < STEP; ++j) {
-        const int it = s * STEP + j, v = vector(it), c = v * VEC - phase;
-        if (it >= n_it || v >= n_vec) continue;
-        uint4* slot = slots + it * VR_THREADS + threadIdx.x;
-        if (c >= 0 && c + VEC <= vocab) {
-          cp_async_16(smem_u32(slot), row + c);
-        } else {
-          T* e = (T*)slot;
-          for (int i = 0; i < VEC; ++i) e[i] = c + i >= 0 && c + i < vocab ? row[c + i] : from_f32<T>(-INFINITY);
+        for (int j = 0; j < STEP; ++j) {
+          const int it = tid * STEP + j, v0 = max(first_vector(it), first_whole), v1 = min(first_vector(it) + VR_THREADS, end_whole);
+          if (it < n_it && v1 > v0) bytes += (uint32_t)(v1 - v0) * 16;
+        }
+        mbar_expect_tx(bars + tid, bytes);
+#pragma unroll
+        for (int j = 0; j < STEP; ++j) {
+          const int it = tid * STEP + j, v0 = max(first_vector(it), first_whole), v1 = min(first_vector(it) + VR_THREADS, end_whole);
+          if (it < n_it && v1 > v0)
+            bulk_load_1d(slots + it * VR_THREADS + (v0 - first_vector(it)), row + (v0 * VEC - phase), (uint32_t)(v1 - v0) * 16, bars + tid);
         }
       }
-      cp_async_commit();
+    } else if (tid == 32 || tid == 64) {  // the vectors that stick out, element by element
+      const int v = tid == 32 ? 0 : n_vec - 1, c = v * VEC - phase, block = v / VR_THREADS;
+      if (block % size == rank && (c < 0 || c + VEC > vocab)) {
+        T* e = (T*)(slots + block / size * VR_THREADS + v % VR_THREADS);
+        for (int i = 0; i < VEC; ++i) e[i] = c + i >= 0 && c + i < vocab ? row[c + i] : from_f32<T>(-INFINITY);
+      }
     }
   }
-  __device__ __forceinline__ void wait(int step) const { cp_async_wait_n(n_steps - 1 - step); }
+  __device__ __forceinline__ void wait(int step) const {
+    if (!mbar_try_wait(bars + step, 0)) row_wait_slow(bars + step, status);
+  }
+  // whether every thread has all of its elements in this step: only the row's last block may be short
+  __device__ __forceinline__ bool whole(int step) const { return (step + 1) * STEP < n_it; }
   // the 16 elements of a step, -inf where the thread has none
+  template <bool WHOLE>
   __device__ __forceinline__ void get(int step, float (&x)[16]) const {
 #pragma unroll
     for (int j = 0; j < STEP; ++j) {
       const int it = step * STEP + j;
-      if (it < n_it && vector(it) < n_vec) {
+      if (WHOLE || (it < n_it && first_vector(it) + (int)threadIdx.x < n_vec)) {
         unpack(slots[it * VR_THREADS + threadIdx.x], x + j * VEC);
       } else {
 #pragma unroll
         for (int i = 0; i < VEC; ++i) x[j * VEC + i] = -INFINITY;
       }
     }
+  }
+  __device__ __forceinline__ void get(int step, float (&x)[16]) const {
+    if (whole(step)) get<true>(step, x);
+    else get<false>(step, x);
   }
   static __device__ __forceinline__ void unpack(const uint4& u, float* x) {
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
@@ -222,6 +254,17 @@ __device__ __forceinline__ bool vectors_aligned(const O* out, int phase) {
   return ((uintptr_t)out - (uintptr_t)phase * sizeof(O)) % (VEC * sizeof(O) < 16 ? VEC * sizeof(O) : 16) == 0;
 }
 
+// Writes a step's results: x[i] belongs to the element that get() gave as x[i].
+template <class O, class T>
+__device__ __forceinline__ void put_step(const RowPart<T>& part, int step, O* out, bool aligned, const float (&x)[16]) {
+  constexpr int VEC = RowPart<T>::VEC;
+#pragma unroll
+  for (int j = 0; j < RowPart<T>::STEP; ++j) {
+    const int it = step * RowPart<T>::STEP + j;
+    if (it < part.n_it) put_vector<O, VEC>(out, part.column(it, threadIdx.x), part.vocab, aligned, x + j * VEC);
+  }
+}
+
 // A running maximum, and the sum of exponentials relative to it.
 struct MaxSum {
   float m = -INFINITY, s = 0.0f;
@@ -241,12 +284,19 @@ struct MaxSum {
     s += (p[0] + p[1]) + (p[2] + p[3]);
   }
 };
-// Sums of several threads' or warps' exponentials, each relative to its own maximum, relative to the maximum of all
-// (a warp's worth; lanes that have none bring m = -inf).
-__device__ __forceinline__ double warp_join(float m, double s, const ExpT& ex, float* m_all) {
-  const float top = warp_max_nan(m);
-  *m_all = top;
-  return warp_sum_f64(m > -INFINITY ? s * (double)ex(m - top) : 0.0);
+// The warp's sum of its threads' exponentials, relative to the largest of their maxima.  In 32 bits: five roundings, which differ from
+// warp to warp; what comes after is in 64.
+__device__ __forceinline__ float warp_join(const MaxSum& t, const ExpT& ex, float* m) {
+  *m = warp_max_nan(t.m);
+  float s = t.m > -INFINITY ? t.s * ex(t.m - *m) : 0.0f;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  return s;
+}
+// The row's sum from the warps' (two a lane; a lane without brings m = -inf).
+__device__ __forceinline__ double cluster_join(float ma, float sa, float mb, float sb, const ExpT& ex, float* m) {
+  *m = warp_max_nan(max_nan(ma, mb));
+  return warp_sum_f64((ma > -INFINITY ? (double)sa * ex(ma - *m) : 0.0) + (mb > -INFINITY ? (double)sb * ex(mb - *m) : 0.0));
 }
 
 // How a row is held: the cluster's CTAs, a power of two, as few as leave a thread with VR_SLOTS vectors at most (three CTAs then
