@@ -1,17 +1,15 @@
-// The k largest logits of each row, in order, with their log-probabilities: a cluster of CTAs a row, which holds the row in shared
-// memory.  Which elements can be among the k largest follows from the threads' maxima, which the pass over the exponentials
-// finds anyway: if every one of W warps has j = ceil(k / W) threads with a maximum of at least x, then k elements are at least x.
-// The elements from there up, a few times k of them, go to the cluster's first CTA, which ranks each by counting the larger ones.
-// Only where they are too many (values that tie, masked rows) is a bound sought that leaves fewer, by bisection over values and
-// indices.
+// The k largest logits of each row, in order, with their log-probabilities: each element read once, by a CTA a row, or by a cluster
+// where there are few rows.  While the row streams by, elements from a bound up are kept, and the bound rises: it is a value that k
+// threads' maxima so far reach, so that k elements reach it.  A warp's few largest maxima are sample enough to find one that not many
+// more reach; it is looked for a few times, and several times k elements are kept on the way.  In the end what reaches the
+// last bound, some more than k, goes to every CTA of the cluster, and each is ranked, by the CTA that found it, by
+// counting the larger ones.  Only where elements kept or left are too many (values that tie, masked rows, rows in ascending order) the row
+// is read again, for a better bound by bisection over values and indices.
 #include "vocab_rows.cuh"
-#include <algorithm>
 
 namespace rt {
 
-constexpr int TOP_ROOM = 2048;  // candidates
-// slots of the row's region at least: it takes the candidates once more when the row is no longer needed
-constexpr int TOP_LEAST_SLOTS = TOP_ROOM / 2 + 1;
+constexpr int TOP_KEPT = 3072, TOP_ROOM = 2048;  // elements that are kept on the way, and that are ranked, at most
 static_assert(TOP_ROOM / VR_MAX_CLUSTER >= RT_TOP_MAX, "k elements of one CTA's share have to fit");
 // An element as an integer, all different: its value's order above, the lower index in front.
 constexpr int TOP_INDEX_BITS = 19;
@@ -21,9 +19,8 @@ __device__ __forceinline__ TopKey top_key(float v, int c) {
   return ((TopKey)order32(v) << TOP_INDEX_BITS) | (uint32_t)((1 << TOP_INDEX_BITS) - 1 - c);
 }
 
-struct TopStat {
+struct alignas(8) TopStat {
   float m, s;
-  uint32_t each, own;  // what every warp of the cluster, and every warp of this CTA, has to have for k elements
 };
 
 // the lanes' values in descending order
@@ -34,195 +31,284 @@ __device__ __forceinline__ uint32_t warp_sort(uint32_t v) {
 #pragma unroll
     for (int stride = size / 2; stride > 0; stride /= 2) {
       const uint32_t o = __shfl_xor_sync(0xffffffffu, v, stride);
-      const bool keep_max = ((lane & stride) == 0) == ((lane & size) == 0 || size == 32);
+      const bool keep_max = ((lane & stride) == 0) == ((lane & size) == 0);
       v = keep_max ? max(v, o) : min(v, o);
     }
   }
   return v;
 }
 
-template <class T>
-__global__ void __launch_bounds__(VR_THREADS, 2) top_logits_kernel(const T* z, size_t ld, int vocab, float t, ExpT ex, int k, int* index, float* logp, float* lse, int* status) {
-  constexpr int VEC = RowPart<T>::VEC, STEP = RowPart<T>::STEP;
-  extern __shared__ uint4 slots[];
-  __shared__ uint64_t bars[VR_MAX_STEPS];
-  __shared__ TopStat stat[VR_MAX_CLUSTER * VR_WARPS];
-  __shared__ int s_n, s_count[2], counts[2][VR_MAX_CLUSTER];
-  __shared__ double s_log_sum;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  cluster_arrive_relaxed();
-  const size_t r = cluster_id();
-  const RowPart<T> part(z + r * ld, vocab, slots, bars, status);
-  part.load();
-  TopKey* room = (TopKey*)(slots + max(part.n_it_most() * VR_THREADS, TOP_LEAST_SLOTS));
-  const int room_each = TOP_ROOM / part.size;
-  if (tid == 0) s_n = s_count[0] = s_count[1] = 0;
-  __syncthreads();
-  MaxSum ms;
-  for (int s = 0; s < part.n_steps; ++s) {
-    float x[16];
-    part.wait(s);
-    part.get(s, x);
-    ms.take(x, ex);
-  }
-  const uint32_t my_top = order32(ms.m), sorted = warp_sort(my_top);
-  const int warps = part.size * VR_WARPS;
-  TopStat st;
-  st.each = __shfl_sync(0xffffffffu, sorted, (k + warps - 1) / warps - 1);
-  st.own = __shfl_sync(0xffffffffu, sorted, (k + VR_WARPS - 1) / VR_WARPS - 1);
-  st.s = warp_join(ms, ex, &st.m);
-  cluster_wait();  // the other CTAs run: their shared memory may be written
-  if (lane < part.size) {
-    const uint32_t to = mapa_u32(smem_u32(&stat[part.rank * VR_WARPS + warp]), lane);
-    st_cluster(to, __float_as_uint(st.m), __float_as_uint(st.s));
-    st_cluster(to + 8, st.each, st.own);
-  }
-  cluster_arrive();
-  cluster_wait();
-  const TopStat none{-INFINITY, 0.0f, 0xffffffffu, 0xffffffffu}, a = lane < warps ? stat[lane] : none, b = lane + 32 < warps ? stat[lane + 32] : none;
-  uint32_t own = a.own, own_b = b.own;  // eight neighbours are a CTA's warps
-#pragma unroll
-  for (int o = 1; o < VR_WARPS; o *= 2) {
-    own = min(own, __shfl_xor_sync(0xffffffffu, own, o));
-    own_b = min(own_b, __shfl_xor_sync(0xffffffffu, own_b, o));
-  }
-  const uint32_t own_max = __reduce_max_sync(0xffffffffu, max(lane < warps ? own : 0u, lane + 32 < warps ? own_b : 0u));
-  const uint32_t bound = max(__reduce_min_sync(0xffffffffu, min(a.each, b.each)), own_max);
-  float m;
-  const double sum = cluster_join(a.m, a.s, b.m, b.s, ex, &m);
-
-  const uint32_t leader_room = mapa_u32(smem_u32(room), 0);
-  auto push = [&](TopKey key) {
-    const int p = atomicAdd(&s_n, 1);
-    if (p < room_each) st_cluster(leader_room + (uint32_t)(part.rank * room_each + p) * 8, key);
-  };
-  if (my_top >= bound) {  // a few threads of a warp, which look for their elements side by side
-    const float from = order32_value(bound);
-    for (int it = 0; it < part.n_it; ++it) {
-      const int c0 = part.column(it, tid);
-      if (c0 >= vocab) break;
-      float x[VEC];
-      RowPart<T>::unpack(slots[it * VR_THREADS + tid], x);
-#pragma unroll
-      for (int i = 0; i < VEC; ++i)
-        if (!(x[i] < from) && c0 + i >= 0 && c0 + i < vocab) push(top_key(x[i], c0 + i));  // NaN too
+// A running reference, and the sum of exponentials relative to it.  It changes when an element is 2^60 times as large, so rarely.
+struct RunningSum {
+  float m = -INFINITY;
+  F2 s[2] = {0, 0};
+  __device__ __forceinline__ void take(const float (&x)[16], float largest, float most, const ExpT& ex) {
+    if (!(largest <= m + most) && m == m) {  // the first finite ones, ones that are far larger, a NaN, which stays
+      const float by = m > -INFINITY ? ex(m - largest) : 0.0f;
+      s[0] = mul2(s[0], pack2(by, by));
+      s[1] = mul2(s[1], pack2(by, by));
+      m = largest;
     }
-  }
-  // every CTA learns how many each has: `to` is written in all of them
-  auto tell = [&](int* to, int n) {
-    if (tid < part.size) st_cluster(mapa_u32(smem_u32(to + part.rank), tid), n);
-    cluster_arrive();
-    cluster_wait();
-  };
-  __syncthreads();
-  tell(counts[0], s_n);
-  bool fits = true;
-  for (int i = 0; i < part.size; ++i) fits &= counts[0][i] <= room_each;
-  if (!fits) {
-    // elements that are at least `key`, in all, and whether every CTA's have room
-    int round = 0;
-    auto count = [&](TopKey key, bool* room_for_all) {
-      const int at = ++round & 1;
-      int n = 0;
-      for (int s = 0; s < part.n_steps; ++s) {
-        float x[16];
-        part.get(s, x);
+    const float ref = m > -INFINITY ? m : 0.0f;
+    const F2 minus_ref = pack2(-ref, -ref);
+    F2 acc[2] = {0, 0};
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int c = part.column(s * STEP + i / VEC, tid) + i % VEC;
-          n += c >= 0 && c < vocab && s * STEP + i / VEC < part.n_it && top_key(x[i], c) >= key;
+    for (int i = 0; i < 16; i += 2) {
+      float a, b;
+      ex.pair(pack2(x[i], x[i + 1]), minus_ref, &a, &b);
+      acc[i / 2 & 1] = add2(acc[i / 2 & 1], pack2(a, b));
+    }
+    s[0] = add2(s[0], acc[0]);
+    s[1] = add2(s[1], acc[1]);
+  }
+};
+
+template <class T, int NT>
+__global__ void __launch_bounds__(NT + 32, ctas_of(NT))
+top_logits_kernel(const T* z, size_t ld, size_t rows, int vocab, float t, ExpT ex, int k, int* index, float* logp, float* lse, int places, int* status) {
+  using Part = RowPart<T, NT>;
+  constexpr int VEC = Part::VEC, STEP = Part::STEP, WARPS = NT / 32, SAMPLE_LANE = (RT_TOP_MAX + 2 * WARPS + 31) / 32;
+  extern __shared__ uint4 slots[];
+  __shared__ uint64_t bars[2 * VR_MAX_BLOCKS + 2];
+  __shared__ TopStat stats[2][VR_MAX_CLUSTER * WARPS];
+  __shared__ uint2 told[2][VR_MAX_CLUSTER];  // what every CTA told
+  __shared__ uint32_t sample[32 * SAMPLE_LANE];
+  __shared__ double s_log_sum;
+  __shared__ int s_kept, s_n, s_count[2], s_found[VR_MAX_CLUSTER];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (tid == 0) s_kept = s_n = s_count[0] = s_count[1] = 0;
+  Exchange exchange;
+  Ring<T, NT> ring(slots + (TOP_KEPT + TOP_ROOM) / 2, bars, places, status, z, ld, rows, vocab, exchange);
+  if (tid >= NT) {
+    if (tid == NT) ring.copy_rows();
+    return;
+  }
+  const double inv_t = 1.0 / t;
+  const float most = 60.0f / ex.hi;
+  // values of a warp in the sample: W warps send at most W + k + W of them
+  const int each = min((k + WARPS - 1) / WARPS + 1, 32), warps = ring.size * WARPS;
+  TopKey *kept = (TopKey*)slots, *room = kept + TOP_KEPT;
+  const int room_each = TOP_ROOM / ring.size;
+  // A value that k of the threads' maxima reach, and not many more of the sample's, in every warp the same.
+  auto bound_of = [&](float largest) {
+    const uint32_t sorted = warp_sort(order32(largest));
+    work_sync<NT>();  // the last one's sample has been read
+    if (lane < each) sample[warp * each + lane] = sorted;
+    work_sync<NT>();
+    uint32_t some[SAMPLE_LANE], lo = 0xffffffffu, hi = 0;  // lo is reached by k; no value is above hi
+#pragma unroll
+    for (int i = 0; i < SAMPLE_LANE; ++i) {
+      const bool on = i * 32 + lane < WARPS * each;
+      some[i] = on ? sample[i * 32 + lane] : 0;
+      if (on) lo = min(lo, some[i]);
+      hi = max(hi, some[i]);
+    }
+    lo = __reduce_min_sync(0xffffffffu, lo);
+    hi = __reduce_max_sync(0xffffffffu, hi);
+    while (hi > lo) {  // at most 32 times
+      const uint32_t mid = lo + (hi - lo) / 2 + 1;
+      int n = 0;
+#pragma unroll
+      for (int i = 0; i < SAMPLE_LANE; ++i)
+        if (i * 32 < WARPS * each) n += some[i] >= mid;
+      n = __reduce_add_sync(0xffffffffu, n);
+      if (n >= k) lo = mid;
+      else hi = mid - 1;
+      if (n >= k && n <= k + k / 8 + 2) break;
+    }
+    return lo;
+  };
+  // Two numbers of every CTA, in every one of them.
+  auto tell = [&](uint32_t a, uint32_t b) {
+    uint2* to = told[exchange.turn()];
+    if (tid == 0) exchange.expect(ring.size * 8);
+    if (tid < ring.size) send(mapa_u32(smem_u32(to + ring.rank), tid), exchange.bar(tid), a, b);
+    exchange.wait();
+    return (const uint2*)to;
+  };
+  for (size_t r = cluster_id(); r < rows; r += ring.row_step) {
+    const Part part = ring.part(r);
+    RunningSum sum;
+    float largest = -INFINITY;  // of the thread's elements
+    uint32_t bound = 0xffffffffu;
+    float from = NAN;
+    auto set_bound = [&](uint32_t b) {
+      bound = b;
+      from = order32_value(b);
+    };
+    const int n_steps = (part.n_it + STEP - 1) / STEP;
+    for (int s = 0; s < n_steps; ++s) {
+      float x[16];
+      const int read = min((s + 1) * STEP, part.n_it) - s * STEP;
+#pragma unroll
+      for (int j = 0; j < STEP; ++j) {
+        const int it = s * STEP + j;
+        if (j < read) {
+          ring.wait(it);
+          if (part.outer(it)) {
+            ring.complete(part, it);
+            fence_proxy_async_smem();  // what it wrote comes before the copies that follow
+          }
+          Part::unpack(ring.block(it)[tid], x + j * VEC);
+        } else {
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) x[j * VEC + i] = -INFINITY;
         }
       }
-      n = __reduce_add_sync(0xffffffffu, n);
-      if (lane == 0) atomicAdd(&s_count[at], n);
-      __syncthreads();
-      const int mine = s_count[at];
-      tell(counts[at], mine);
-      if (tid == 0) s_count[at] = 0;  // before the barrier inside the next round, which uses the other one
-      n = 0;
-      *room_for_all = true;
-      for (int i = 0; i < part.size; ++i) {
-        n += counts[at][i];
-        *room_for_all &= counts[at][i] <= room_each;
-      }
-      return n;
-    };
-    // lo is reached by k elements, hi by fewer; elements are all different, so that some key between is reached by exactly k
-    TopKey lo = (TopKey)bound << TOP_INDEX_BITS, hi = (TopKey)1 << (32 + TOP_INDEX_BITS);
-    bool room_for_all = false;
-    for (TopKey mid = min(lo + ((TopKey)1 << TOP_INDEX_BITS), hi - 1); !room_for_all; mid = lo + (hi - lo) / 2) {  // first: are the bound's ties the matter?
-      const int n = count(mid, &room_for_all);
-      room_for_all &= n >= k;
-      if (n >= k) lo = mid;
-      else hi = mid;
-    }
-    if (tid == 0) s_n = 0;
-    __syncthreads();
-    for (int s = 0; s < part.n_steps; ++s) {
-      float x[16];
-      part.get(s, x);
+      __syncwarp();
+      if (lane < read) mbar_arrive(ring.empty + ring.place(s * STEP + lane));
+      float top = max_nan(x[0], x[1], x[2]);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int c = part.column(s * STEP + i / VEC, tid) + i % VEC;
-        if (c >= 0 && c < vocab && s * STEP + i / VEC < part.n_it && top_key(x[i], c) >= lo) push(top_key(x[i], c));
+      for (int i = 3; i < 15; i += 2) top = max_nan(top, x[i], x[i + 1]);
+      top = max_nan(top, x[15]);
+      sum.take(x, top, most, ex);
+      largest = max_nan(largest, top);
+      // for a bound: after 1, 4, 16 ... steps (1, 2, 4, 8 ... for long lists), but not shortly before the end
+      if ((s & (s + 1)) == 0 && (k > 64 || (s + 1) % 3 == 1) && (s == 0 || (s + 1) * 4 < n_steps * 3)) {
+        set_bound(bound_of(largest));
+        if (*(volatile int*)&s_kept > TOP_KEPT) from = INFINITY;  // too many already: none any more
       }
+      if (!(top < from)) {  // NaN too
+        if (*(volatile int*)&s_kept <= TOP_KEPT) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            if (x[i] < from) continue;
+            const int it = s * STEP + i / VEC, c = part.column(it) + i % VEC;
+            if (it >= part.n_it || c < 0 || c >= vocab) continue;
+            const int p = atomicAdd(&s_kept, 1);
+            if (p < TOP_KEPT) kept[p] = top_key(x[i], c);
+          }
+        }
+      }
+      ring.advance(read, s + 1 == n_steps);
     }
-    __syncthreads();
-    tell(counts[++round & 1], s_n);
-    if (tid < part.size) counts[0][tid] = counts[round & 1][tid];
-    __syncthreads();
-  }
-  if (part.rank != 0) return;
-  const bool bad = !(m < INFINITY);
-  if (tid == 0) {
-    s_log_sum = log(sum);
-    if (lse) lse[r] = bad ? NAN : (float)((double)m / t + s_log_sum);
-  }
-  __syncthreads();
-  // The lists one behind the other in what held the row: orders, filled up with the lowest to a multiple of four, and columns.
-  int n = 0;
-  for (int l = 0; l < part.size; ++l) n += counts[0][l];
-  const int n4 = (n + 3) / 4;
-  uint32_t *order = (uint32_t*)slots, *column = order + 4 * n4;
-  int before = 0;
-  for (int l = 0; l < part.size; ++l) {
-    const int here = counts[0][l];
-    for (int i = tid; i < here; i += VR_THREADS) {
-      const TopKey key = room[l * room_each + i];
-      order[before + i] = (uint32_t)(key >> TOP_INDEX_BITS);
-      column[before + i] = (1 << TOP_INDEX_BITS) - 1 - (uint32_t)(key & ((1 << TOP_INDEX_BITS) - 1));
+    set_bound(bound_of(largest));
+    TopStat st;
+    float a, b;
+    unpack2(add2(sum.s[0], sum.s[1]), &a, &b);
+    st.s = warp_join(sum.m, a + b, ex, &st.m);
+    TopStat* stat = stats[exchange.turn()];
+    uint2* to = told[exchange.turn()];
+    const int n_kept = s_kept;  // all have been counted before the bound's barriers
+    if (tid == 0) exchange.expect(warps * sizeof(TopStat) + ring.size * 8);
+    if (lane < ring.size) send(mapa_u32(smem_u32(&stat[ring.rank * WARPS + warp]), lane), exchange.bar(lane), __float_as_uint(st.m), __float_as_uint(st.s));
+    if (tid < ring.size) send(mapa_u32(smem_u32(to + ring.rank), tid), exchange.bar(tid), bound, (uint32_t)n_kept);
+    exchange.wait();
+    float m;
+    const double lane_sum = lane_join(warps, [&](int i, float* mi, float* si) { *mi = stat[i].m, *si = stat[i].s; }, ex, &m);
+    if (warp == WARPS - 1) {
+      const double all = warp_sum_f64(lane_sum);
+      if (lane == 0) s_log_sum = log(all);
     }
-    before += here;
-  }
-  if (tid < 4 * n4 - n) order[n + tid] = 0;
-  __syncthreads();
-  const double log_sum = s_log_sum;
-  for (int i = tid; i < n; i += VR_THREADS) {
-    const uint32_t mine = order[i];
-    int rank = 0, same = -1;
-#pragma unroll 4
-    for (int j = 0; j < n4; ++j) {
-      const uint4 o = ((const uint4*)order)[j];
-      rank += (o.x > mine) + (o.y > mine) + (o.z > mine) + (o.w > mine);
-      same += (o.x == mine) + (o.y == mine) + (o.z == mine) + (o.w == mine);
+    bool fits = true;
+    for (int i = 0; i < ring.size; ++i) {  // every CTA's bound holds for the row
+      fits &= to[i].y <= (uint32_t)TOP_KEPT;
+      bound = max(bound, to[i].x);
     }
-    if (rank >= k) continue;
-    if (same > 0)
-      for (int j = 0; j < n; ++j) rank += order[j] == mine && column[j] < column[i];
-    if (rank >= k) continue;
-    const float v = order32_value(mine);
-    index[r * k + rank] = (int)column[i];
-    logp[r * k + rank] = bad ? NAN : v == -INFINITY ? -INFINITY : (float)(((double)v - m) / t - log_sum);
+    // elements to be ranked: this CTA's lie in its share of the room
+    TopKey* mine = room + ring.rank * room_each;
+    auto push = [&](TopKey key) {
+      const int p = atomicAdd(&s_n, 1);
+      if (p < room_each) mine[p] = key;
+    };
+    if (fits) {
+      for (int i = tid; i < n_kept; i += NT)
+        if (kept[i] >= (TopKey)bound << TOP_INDEX_BITS) push(kept[i]);
+    }
+    work_sync<NT>();
+    const uint2* found = tell((uint32_t)s_n, 0);
+    for (int i = 0; i < ring.size; ++i) fits &= found[i].x <= (uint32_t)room_each;
+    if (!fits) {
+      auto each_element = [&](auto&& f) {
+#pragma unroll 1
+        for (int it = 0; it < part.n_it; ++it) {
+          const int c0 = part.column(it);
+          for (int c = max(c0, 0); c < min(c0 + VEC, vocab); ++c) f(to_f32(part.row[c]), c);
+        }
+      };
+      // elements that are at least `key`, in all, and whether every CTA's have room
+      int round = 0;
+      auto count = [&](TopKey key, bool* room_for_all) {
+        const int now = ++round & 1;
+        int n = 0;
+        each_element([&](float v, int c) { n += top_key(v, c) >= key; });
+        n = __reduce_add_sync(0xffffffffu, n);
+        if (lane == 0) atomicAdd(&s_count[now], n);
+        work_sync<NT>();
+        const uint2* counts = tell((uint32_t)s_count[now], 0);
+        n = 0;
+        *room_for_all = true;
+        for (int i = 0; i < ring.size; ++i) {
+          n += (int)counts[i].x;
+          *room_for_all &= counts[i].x <= (uint32_t)room_each;
+        }
+        work_sync<NT>();
+        if (tid == 0) s_count[now] = 0;  // before the barrier of the next round, which uses the other one
+        return n;
+      };
+      // low is reached by k elements, high by fewer; elements are all different, so that some key between is reached by exactly k
+      TopKey low = (TopKey)bound << TOP_INDEX_BITS, high = (TopKey)1 << (32 + TOP_INDEX_BITS);
+      bool room_for_all = false;
+      // the first question: are the bound's ties the matter?
+      for (TopKey mid = min(low + ((TopKey)1 << TOP_INDEX_BITS), high - 1); !room_for_all; mid = low + (high - low) / 2) {
+        const int n = count(mid, &room_for_all);
+        room_for_all &= n >= k;
+        if (n >= k) low = mid;
+        else high = mid;
+      }
+      if (tid == 0) s_n = 0;
+      work_sync<NT>();
+      each_element([&](float v, int c) {
+        if (top_key(v, c) >= low) push(top_key(v, c));
+      });
+      work_sync<NT>();
+      found = tell((uint32_t)s_n, 0);
+    }
+    const int n_mine = (int)found[ring.rank].x;
+    if (ring.size > 1) {  // everybody's to everybody
+      int n = 0;
+      for (int i = 0; i < ring.size; ++i) n += (int)found[i].x;
+      if (tid < ring.size) s_found[tid] = (int)found[tid].x;  // what was told may be overwritten once this exchange is over
+      work_sync<NT>();
+      if (tid == 0) exchange.expect((uint32_t)(n - n_mine) * 8);
+      for (int i = tid; i < n_mine; i += NT) {
+        const uint2 key = *(const uint2*)(mine + i);
+        for (int o = 0; o < ring.size; ++o)
+          if (o != ring.rank) send(mapa_u32(smem_u32(mine + i), o), exchange.bar(o), key.x, key.y);
+      }
+      exchange.wait();
+    }
+    const bool bad = !(m < INFINITY);
+    const double log_sum = s_log_sum;
+    if (lse && tid == 0 && ring.rank == 0) lse[r] = bad ? NAN : (float)(m * inv_t + log_sum);
+    // a warp an element: its rank is the number of larger ones
+    for (int i = warp; i < n_mine; i += WARPS) {
+      const TopKey key = mine[i];
+      int rank = 0;
+      for (int o = 0; o < ring.size; ++o) {
+        const int n = ring.size > 1 ? s_found[o] : n_mine;
+        for (int j = lane; j < n; j += 32) rank += room[o * room_each + j] > key;
+      }
+      rank = __reduce_add_sync(0xffffffffu, rank);
+      if (rank >= k || lane > 0) continue;
+      const float v = order32_value((uint32_t)(key >> TOP_INDEX_BITS));
+      index[r * k + rank] = (1 << TOP_INDEX_BITS) - 1 - (int)(key & ((1 << TOP_INDEX_BITS) - 1));
+      logp[r * k + rank] = bad ? NAN : v == -INFINITY ? -INFINITY : (float)(((double)v - m) * inv_t - log_sum);
+    }
+    work_sync<NT>();
+    if (tid == 0) s_n = s_kept = 0;  // the next row's first bound has barriers before they count again
   }
 }
 
 int launch_top_logits(rt_ctx* c, const VocabRows& z, size_t rows, int vocab, float temperature, int k, int* index, float* logp, float* lse) {
-  const RowShape shape = row_shape(vocab, z.dtype);
-  const size_t smem = std::max(shape.slots, (size_t)TOP_LEAST_SLOTS) * 16 + TOP_ROOM * 8;
+  // long lists want more threads, whose maxima are the sample that the bound is found in
+  const RowShape shape = stream_shape(c, rows, vocab, z.dtype, k <= 64 ? 256 : 512, (TOP_KEPT + TOP_ROOM) * sizeof(TopKey));
   return with_dtype(z.dtype, [&](auto* zt) {
-    using T = std::remove_pointer_t<decltype(zt)>;
-    return launch_clusters(c, top_logits_kernel<T>, rows, shape.cluster, smem, (const T*)z.p, z.ld, vocab, temperature,
-                           exp_t(temperature), k, index, logp, lse, c->status_dev);
+    return with_threads(shape.threads, [&](auto threads) {
+      using T = std::remove_pointer_t<decltype(zt)>;
+      return launch_clusters(c, top_logits_kernel<T, decltype(threads)::value>, true, rows, shape.threads + 32, shape.cluster, shape.smem, (const T*)z.p, z.ld,
+                             rows, vocab, temperature, exp_t(temperature), k, index, logp, lse, shape.places, c->status_dev);
+    });
   });
 }
 

@@ -5,7 +5,14 @@
 
 namespace rt {
 
-constexpr int VD_EIGHTHS = 8;
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_arrive_relaxed() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ void st_cluster(uint32_t addr, double v) {
+  asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(addr), "d"(v) : "memory");
+}
+
+constexpr int VD_THREADS = 256, VD_WARPS = VD_THREADS / 32, VD_EIGHTHS = 8;
 
 __device__ __forceinline__ bool is_mass(float v) { return v > 0.0f && v < INFINITY; }
 
@@ -57,8 +64,8 @@ struct Left {
   // the masses as sums of two floats: a difference of two floats is one rounded and what the rounding lost
   __device__ __forceinline__ void masses(int v, const uint4& a, const uint4& b, float (&x)[VEC], float (&lo)[VEC]) const {
     float pa[VEC], pb[VEC];
-    RowPart<T>::unpack(a, pa);
-    RowPart<T>::unpack(b, pb);
+    unpack_vector<T>(a, pa);
+    unpack_vector<T>(b, pb);
     const int skip = without - column(v);
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
@@ -71,12 +78,12 @@ struct Left {
 };
 
 template <class T>
-__global__ void __launch_bounds__(VR_THREADS) verify_draft_kernel(const T* P, size_t ld_p, const T* Q, size_t ld_q, int vocab, const int* tok,
+__global__ void __launch_bounds__(VD_THREADS) verify_draft_kernel(const T* P, size_t ld_p, const T* Q, size_t ld_q, int vocab, const int* tok,
                                                                   const int* offsets, int n_seq, int n_draft, const float* u_accept,
                                                                   const float* u_sample, int* accepted, int* token, int* status) {
   constexpr int VEC = Left<T>::VEC;
   __shared__ int s_first, s_bad;
-  __shared__ double mass[2][VR_MAX_CLUSTER * VR_WARPS];
+  __shared__ double mass[2][VR_MAX_CLUSTER * VD_WARPS];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = (int)cluster_ctarank(), size = (int)cluster_size();
   const int s = (int)cluster_id();
   cluster_arrive_relaxed();
@@ -86,7 +93,7 @@ __global__ void __launch_bounds__(VR_THREADS) verify_draft_kernel(const T* P, si
   __syncthreads();
   bool bad = a < 0 || e < a || e > n_draft || (s == 0 && a != 0) || (s == n_seq - 1 && e != n_draft);
   if (!bad)
-    for (int i = a + tid; i < e; i += VR_THREADS) {
+    for (int i = a + tid; i < e; i += VD_THREADS) {
       const int d = tok[i];
       if (d < 0 || d >= vocab) { s_bad = 1; continue; }
       const double p = to_f32(P[(size_t)(i + s) * ld_p + d]), q = Q ? to_f32(Q[(size_t)i * ld_q + d]) : 1.0;
@@ -105,7 +112,7 @@ __global__ void __launch_bounds__(VR_THREADS) verify_draft_kernel(const T* P, si
   }
   const int at = min(s_first, e);
   if (tid == 0 && rank == 0) accepted[s] = at - a;
-  const int pieces = size * VR_WARPS, piece = rank * VR_WARPS + warp;
+  const int pieces = size * VD_WARPS, piece = rank * VD_WARPS + warp;
   const T* p_row = P + (size_t)(at + s) * ld_p;
   Left<T> left(p_row, Q && at < e ? Q + (size_t)at * ld_q : nullptr, !Q && at < e ? tok[at] : -1, vocab);
   // vectors of an eighth of a piece, in rounds of a warp
@@ -219,7 +226,7 @@ int launch_verify_draft(rt_ctx* c, const VerifyArgs& a) {
   const int size = a.vocab >= 8192 ? 8 : a.vocab >= 2048 ? 2 : 1;
   return with_dtype(a.p.dtype, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    return launch_clusters(c, verify_draft_kernel<T>, a.n_seq, size, 0, (const T*)a.p.p, a.p.ld, (const T*)a.q.p, a.q.ld, a.vocab, a.tok, a.offsets,
+    return launch_clusters(c, verify_draft_kernel<T>, false, a.n_seq, VD_THREADS, size, 0, (const T*)a.p.p, a.p.ld, (const T*)a.q.p, a.q.ld, a.vocab, a.tok, a.offsets,
                            a.n_seq, a.n_draft, a.u_accept, a.u_sample, a.accepted, a.token, c->status_dev);
   });
 }
