@@ -393,6 +393,28 @@ rt_status rt_model_score_layout(rt_model* m, const int32_t* tokens, const int32_
 rt_status rt_model_argmax_layout(rt_model* m, const int32_t* tokens, const int32_t* seq_offsets, int32_t n_seq,
                                  const int32_t* positions, const int32_t* segments, const int32_t* target_pos,
                                  int32_t n_targets, int32_t* argmax_out);
+/* What a teacher hands on (no counterpart in the reference): the k largest logits of every target row of a forward-only
+ * pass, with their log-probabilities and the row's log-sum-exp at a temperature, as rt_top_logits_dev gives them:
+ * index_out, logp_out [n_targets x k], lse_out [n_targets] or NULL.  positions / segments as above.  The teacher may be
+ * another model, or this one with its adapters off. */
+rt_status rt_model_top_logits(rt_model* m, const int32_t* tokens, const int32_t* seq_offsets, int32_t n_seq,
+                              const int32_t* positions, const int32_t* segments, const int32_t* target_pos, int32_t n_targets,
+                              float temperature, int32_t k, int32_t* index_out, float* logp_out, float* lse_out);
+/* The third objective beside SFT and DPO (src/train.rs:269-297 has those; this one has no counterpart): every target row
+ * learns from a teacher's list [n_targets x k] as rt_distill_dev says; adds into every adapter's gradients and writes the
+ * weighted loss of each target. */
+rt_status rt_model_distill_backward(rt_model* m, const int32_t* tokens, const int32_t* seq_offsets, int32_t n_seq,
+                                    const int32_t* positions, const int32_t* segments, const int32_t* target_pos,
+                                    const float* weights, int32_t n_targets, float temperature, int32_t mode, int32_t k,
+                                    const int32_t* index, const float* teacher_logp, float* loss_out);
+/* The sampling counterpart of greedy_prefix (src/eval.rs:152-173): which of the tokens that each sequence holds from
+ * draft_from[s] on (1 <= draft_from[s] <= its length) this model would let stand, drafted by `draft` (another model on the
+ * same context with the same vocabulary) or, with NULL, without probabilities; one forward pass of each over the sequences,
+ * then rt_verify_draft_dev on the softmax of their rows at the temperature.  u_accept has a number for every drafted token,
+ * sequence by sequence.  A sequence drafts fewer tokens than the models' head_rows (else RT_ERR_TOO_LARGE). */
+rt_status rt_model_verify_draft(rt_model* m, rt_model* draft, const int32_t* tokens, const int32_t* seq_offsets, int32_t n_seq,
+                                const int32_t* draft_from, float temperature, const float* u_accept, const float* u_sample,
+                                int32_t* accepted_out, int32_t* token_out);
 /* The same step split for hosts that keep the batch on the device: stage copies tokens,
  * targets and weights to HBM once; run_staged does the forward + backward (backward != 0) or
  * the forward alone on the staged batch without touching host memory; read_results copies the

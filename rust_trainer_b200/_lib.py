@@ -147,6 +147,9 @@ def _declare(L: C.CDLL) -> None:
         "rt_op_top_logits": (i32, [vp, f32p, sz, sz, cf, ci, i32p, f32p, f32p]),
         "rt_op_distill": (i32, [vp, f32p, sz, sz, cf, i32p, f32p, ci, ci, f32p, f32p, f32p]),
         "rt_op_softmax": (i32, [vp, f32p, sz, sz, cf, f32p]),
+        "rt_model_top_logits": (i32, [vp, i32p, i32p, i32, i32p, i32p, i32p, i32, cf, i32, i32p, f32p, f32p]),
+        "rt_model_distill_backward": (i32, [vp, i32p, i32p, i32, i32p, i32p, i32p, f32p, i32, cf, i32, i32, i32p, f32p, f32p]),
+        "rt_model_verify_draft": (i32, [vp, vp, i32p, i32p, i32, i32p, cf, f32p, f32p, i32p, i32p]),
         "rt_op_verify_draft": (i32, [vp, f32p, f32p, sz, i32p, i32p, sz, f32p, f32p, i32p, i32p]),
     })
     for name, (res, args) in sig.items():

@@ -3,6 +3,7 @@
 // sequencing the reference does in src/linear.rs, src/attention.rs, src/model.rs and
 // src/optim.rs, plus buffer management.
 #include "model.h"
+#include "vocab_rows.h"
 #include "pdl.cuh"
 #include <math.h>
 #include <algorithm>
@@ -1245,6 +1246,15 @@ static rt_status block_backward(rt_model* m, int li, int M, const float* x_in, c
   return RT_OK;
 }
 
+// The logits of R target rows from c0 on, in f32 (the head's first half, src/model.rs:561-578).
+static rt_status head_logits(rt_model* m, rt_linear* head, int c0, int R) {
+  const rt_model_config& g = m->cfg;
+  cudaStream_t st = m->ctx->stream;
+  launch_gather_f32_rows(m->x.as<float>(), m->tpos + c0, R, g.hidden, m->xs.as<float>(), st);
+  launch_rmsnorm_fwd(m->xs.as<float>(), m->final_norm, R, g.hidden, g.rms_eps, m->ns16.as<__half>(), st);
+  return linear_forward_dev(head, m->lsc, m->ns16.as<__half>(), R, m->logits.p, RT_DT_F32, 0);
+}
+
 // Model::head (src/model.rs:561-609) in chunks of head_rows targets.
 static rt_status model_head(rt_model* m, int M, int n_targets, bool backward, float* logits_out_host) {
   rt_ctx* c = m->ctx;
@@ -1253,25 +1263,36 @@ static rt_status model_head(rt_model* m, int M, int n_targets, bool backward, fl
   const int d = g.hidden, V = g.vocab;
   (void)M;
   RT_CUDA(c, cudaMemsetAsync(m->hits(), 0, 4, st));
+  if (m->head.kind == rt_model::HEAD_NONE) return RT_OK;
   rt_linear head;  // a bias-free, adapter-free Linear over the lm_head weight
   head.ctx = c;
   head.w = m->lm_head;
   for (int c0 = 0; c0 < n_targets; c0 += g.head_rows) {
-    const int R = n_targets - c0 < g.head_rows ? n_targets - c0 : g.head_rows;
-    const int* tpos = m->tpos + c0;
-    launch_gather_f32_rows(m->x.as<float>(), tpos, R, d, m->xs.as<float>(), st);
-    launch_rmsnorm_fwd(m->xs.as<float>(), m->final_norm, R, d, g.rms_eps, m->ns16.as<__half>(), st);
-    RT_TRY(linear_forward_dev(&head, m->lsc, m->ns16.as<__half>(), R, m->logits.p, RT_DT_F32, 0));
+    const int R = n_targets - c0 < g.head_rows ? n_targets - c0 : g.head_rows, k = m->head.k;
+    const VocabRows rows{m->logits.p, RT_DT_F32, (size_t)V};
+    RT_TRY(head_logits(m, &head, c0, R));
     if (logits_out_host)
       RT_CUDA(c, cudaMemcpyAsync(logits_out_host + (size_t)c0 * V, m->logits.p, (size_t)R * V * 4, cudaMemcpyDeviceToHost, st));
-    if (launch_ce_rows(c, m->logits.as<float>(), R, V, m->ttok + c0, m->tw + c0, m->logp() + c0, m->hits(),
-                       backward ? m->dl16.as<__half>() : nullptr, backward ? m->sc_l.as<float>() : nullptr,
-                       m->want_argmax ? m->argmax.as<int>() + c0 : nullptr))
+    if (m->head.kind == rt_model::HEAD_TOP) {
+      float* logp = m->list_logp();
+      if (launch_top_logits(c, rows, R, V, m->head.temperature, k, m->list_index() + (size_t)c0 * k, logp + (size_t)c0 * k,
+                            logp + (size_t)m->list_targets * k + c0))
+        return c->fail(RT_ERR_CUDA, "top-logits launch failed");
+      continue;
+    }
+    if (m->head.kind == rt_model::HEAD_DISTILL) {
+      const DistillArgs a{rows, V, k, m->head.mode, m->head.temperature, m->list_index() + (size_t)c0 * k, m->list_logp() + (size_t)c0 * k,
+                          m->tw + c0, m->logp() + c0, m->dl16.p, RT_DT_F16, (size_t)V, m->sc_l.as<float>()};
+      if (launch_distill_rows(c, a, R)) return c->fail(RT_ERR_CUDA, "distillation launch failed");
+    } else if (launch_ce_rows(c, m->logits.as<float>(), R, V, m->ttok + c0, m->tw + c0, m->logp() + c0, m->hits(),
+                              backward ? m->dl16.as<__half>() : nullptr, backward ? m->sc_l.as<float>() : nullptr,
+                              m->want_argmax ? m->argmax.as<int>() + c0 : nullptr)) {
       return c->fail(RT_ERR_CUDA, "cross-entropy launch failed");
+    }
     if (backward) {
       RT_TRY(linear_backward_dev(&head, m->lsc, m->ns16.as<__half>(), m->dl16.as<__half>(), m->sc_l.as<float>(), R, m->dns.as<float>(), 0));
       launch_rmsnorm_bwd(m->xs.as<float>(), m->final_norm, m->dns.as<float>(), nullptr, R, d, g.rms_eps, m->dxs.as<float>(), nullptr, nullptr, st);
-      launch_scatter_add_rows(m->dxs.as<float>(), tpos, R, d, m->dx.as<float>(), st);
+      launch_scatter_add_rows(m->dxs.as<float>(), m->tpos + c0, R, d, m->dx.as<float>(), st);
     }
   }
   return RT_OK;
@@ -1415,6 +1436,11 @@ static uint64_t buffer_signature(rt_model* m) {
   mix((const void*)(uintptr_t)m->n_params);
   mix((const void*)(uintptr_t)(m->store_acts ? 1 : 0));
   mix(m->gap);
+  mix(m->lists.p);
+  uint32_t t_bits;
+  memcpy(&t_bits, &m->head.temperature, 4);
+  for (const uint64_t v : {(uint64_t)m->head.kind, (uint64_t)m->head.k, (uint64_t)m->head.mode, (uint64_t)m->list_targets, (uint64_t)t_bits})
+    mix((const void*)(uintptr_t)v);
   for (auto& b : m->blocks)
     for (int i = 0; i < 7; ++i) mix((const void*)(uintptr_t)(b.lin[i]->lora_active() ? b.lin[i]->lora.rank : 0));
   return h;
@@ -1431,7 +1457,8 @@ static rt_status run_staged(rt_model* m, bool backward, float* logits_out_host) 
     const char* e = getenv("RT_B200_NO_GRAPH");
     m->use_graphs = (e && e[0] == '1') ? 0 : 1;
   }
-  if (!m->use_graphs || c->profiling || logits_out_host || m->want_argmax || c->stream == nullptr)
+  if (!m->use_graphs || c->profiling || logits_out_host || m->want_argmax || m->head.kind == rt_model::HEAD_TOP || m->head.kind == rt_model::HEAD_NONE ||
+      c->stream == nullptr)
     return run_staged_body(m, backward, logits_out_host);
   RT_CUDA(c, cudaSetDevice(c->device));
   rt_model::Shape shape{m->staged_tokens, m->staged_targets, backward ? 1 : 0, buffer_signature(m)};
@@ -1584,6 +1611,165 @@ rt_status rt_model_argmax_layout(rt_model* m, const int32_t* tokens, const int32
   if (st) return st;
   RT_CUDA(c, cudaMemcpyAsync(argmax_out, m->argmax.p, (size_t)n_targets * 4, cudaMemcpyDeviceToHost, c->stream));
   return c->check_device_status("rt_model_argmax_layout");
+}
+
+// Sets the head's work for one pass; scoring again afterwards, however the pass ends.
+namespace {
+struct HeadScope {
+  rt_model* m;
+  HeadScope(rt_model* m_, rt_model::HeadKind kind, float temperature, int k, int mode, int n_targets) : m(m_) {
+    m->head.kind = kind;
+    m->head.temperature = temperature;
+    m->head.k = k;
+    m->head.mode = mode;
+    m->list_targets = n_targets;
+  }
+  ~HeadScope() { m->head = {}; m->list_targets = 0; }
+};
+bool bad_temperature(float t) { return !(t >= 1e-4f && t <= 1e4f); }
+}  // namespace
+
+rt_status rt_model_top_logits(rt_model* m, const int32_t* tokens, const int32_t* seq_offsets, int32_t n_seq, const int32_t* positions,
+                              const int32_t* segments, const int32_t* tpos, int32_t n_targets, float temperature, int32_t k, int32_t* index_out,
+                              float* logp_out, float* lse_out) {
+  if (!m || !index_out || !logp_out) return RT_ERR_BAD_ARG;
+  rt_ctx* c = m->ctx;
+  if (n_targets <= 0) return RT_OK;
+  if (n_targets > (1 << 24)) return c->fail(RT_ERR_BAD_SHAPE, "too many targets");
+  if (k < 1 || k > RT_TOP_MAX || k > m->cfg.vocab || m->cfg.vocab > RT_VOCAB_MAX) return c->fail(RT_ERR_BAD_SHAPE, "k or the vocabulary out of range");
+  if (bad_temperature(temperature)) return c->fail(RT_ERR_BAD_ARG, "temperature out of range");
+  std::vector<int32_t> ttok((size_t)n_targets, 0);  // rows are not scored; any valid token does
+  int M = 0;
+  m->staged_tokens = 0;
+  RT_TRY(upload_batch(m, tokens, seq_offsets, n_seq, tpos, ttok.data(), nullptr, n_targets, false, &M, positions, segments));
+  const size_t n = (size_t)n_targets;
+  if (!m->lists.reserve((2 * n * k + n) * 4)) return c->fail(RT_ERR_CUDA, "out of device memory (lists)");
+  m->staged_tokens = M;
+  m->staged_targets = n_targets;
+  m->staged_has_weights = false;
+  const HeadScope scope(m, rt_model::HEAD_TOP, temperature, k, 0, n_targets);
+  RT_TRY(run_staged(m, false, nullptr));
+  RT_CUDA(c, cudaMemcpyAsync(index_out, m->list_index(), n * k * 4, cudaMemcpyDeviceToHost, c->stream));
+  RT_CUDA(c, cudaMemcpyAsync(logp_out, m->list_logp(), n * k * 4, cudaMemcpyDeviceToHost, c->stream));
+  if (lse_out) RT_CUDA(c, cudaMemcpyAsync(lse_out, m->list_logp() + n * k, n * 4, cudaMemcpyDeviceToHost, c->stream));
+  return c->check_device_status("rt_model_top_logits");
+}
+
+rt_status rt_model_distill_backward(rt_model* m, const int32_t* tokens, const int32_t* seq_offsets, int32_t n_seq, const int32_t* positions,
+                                    const int32_t* segments, const int32_t* tpos, const float* weights, int32_t n_targets, float temperature,
+                                    int32_t mode, int32_t k, const int32_t* index, const float* teacher_logp, float* loss_out) {
+  if (!m) return RT_ERR_BAD_ARG;
+  rt_ctx* c = m->ctx;
+  if (n_targets <= 0 || !weights || !index || !teacher_logp || !loss_out) return c->fail(RT_ERR_BAD_ARG, "targets, weights or lists missing");
+  if (n_targets > (1 << 24)) return c->fail(RT_ERR_BAD_SHAPE, "too many targets");
+  if (k < 1 || k > RT_TOP_MAX || m->cfg.vocab > RT_VOCAB_MAX) return c->fail(RT_ERR_BAD_SHAPE, "k or the vocabulary out of range");
+  if (bad_temperature(temperature)) return c->fail(RT_ERR_BAD_ARG, "temperature out of range");
+  if (mode != RT_DISTILL_RENORM && mode != RT_DISTILL_TAIL) return c->fail(RT_ERR_BAD_ARG, "unknown distillation mode");
+  const size_t n = (size_t)n_targets;
+  for (size_t i = 0; i < n * k; ++i)
+    if (index[i] < -1 || index[i] >= m->cfg.vocab) return c->fail(RT_ERR_BAD_INDEX, "listed token out of vocabulary");
+  std::vector<int32_t> ttok(n, 0);
+  int M = 0;
+  m->staged_tokens = 0;
+  RT_TRY(upload_batch(m, tokens, seq_offsets, n_seq, tpos, ttok.data(), weights, n_targets, true, &M, positions, segments));
+  if (!m->lists.reserve((2 * n * k + n) * 4)) return c->fail(RT_ERR_CUDA, "out of device memory (lists)");
+  m->staged_tokens = M;
+  m->staged_targets = n_targets;
+  m->staged_has_weights = true;
+  const HeadScope scope(m, rt_model::HEAD_DISTILL, temperature, k, mode, n_targets);
+  RT_CUDA(c, cudaMemcpyAsync(m->list_index(), index, n * k * 4, cudaMemcpyHostToDevice, c->stream));
+  RT_CUDA(c, cudaMemcpyAsync(m->list_logp(), teacher_logp, n * k * 4, cudaMemcpyHostToDevice, c->stream));
+  rt_status st = run_staged(m, true, nullptr);
+  m->staged_tokens = 0;  // its targets' tokens are none: not to be run as a scoring batch
+  m->staged_has_weights = false;
+  if (st) return st;
+  return rt_model_read_results(m, loss_out, n_targets, nullptr);
+}
+
+rt_status rt_model_verify_draft(rt_model* m, rt_model* draft, const int32_t* tokens, const int32_t* seq_offsets, int32_t n_seq,
+                                const int32_t* draft_from, float temperature, const float* u_accept, const float* u_sample,
+                                int32_t* accepted_out, int32_t* token_out) {
+  if (!m) return RT_ERR_BAD_ARG;
+  rt_ctx* c = m->ctx;
+  if (!tokens || !seq_offsets || n_seq <= 0 || !draft_from || !u_sample || !accepted_out || !token_out) return c->fail(RT_ERR_BAD_ARG, "empty batch");
+  if (draft == m || (draft && (draft->ctx != c || draft->cfg.vocab != m->cfg.vocab)))
+    return c->fail(RT_ERR_BAD_ARG, "the drafting model is another one on the same context, with the same vocabulary");
+  if (m->cfg.vocab > RT_VOCAB_MAX) return c->fail(RT_ERR_BAD_SHAPE, "vocabulary out of range");
+  if (bad_temperature(temperature)) return c->fail(RT_ERR_BAD_ARG, "temperature out of range");
+  const int most = draft && draft->cfg.head_rows < m->cfg.head_rows ? draft->cfg.head_rows : m->cfg.head_rows, total = seq_offsets[n_seq];
+  if (n_seq > (1 << 24) || total <= 0 || total > (1 << 24)) return c->fail(RT_ERR_BAD_SHAPE, "token count out of range");
+  // rows: of the target, the position in front of every draft and the last one; of the drafting model, those in front of drafts
+  std::vector<int32_t> t_pos, d_pos, tok, off(1, 0), first_seq;  // first_seq: of the chunks of whole sequences that the head takes at once
+  int chunk = 0;
+  for (int s = 0; s < n_seq; ++s) {
+    const int a = seq_offsets[s], e = seq_offsets[s + 1], from = draft_from[s];
+    if (a < 0 || e <= a || e > total) return c->fail(RT_ERR_BAD_SHAPE, "empty or unordered sequence");
+    if (from < 1 || from > e - a) return c->fail(RT_ERR_BAD_INDEX, "drafts start behind the sequence's first token, within it or at its end");
+    const int n = e - a - from;
+    if (n + 1 > most) return c->fail(RT_ERR_TOO_LARGE, "more drafts in a sequence than head_rows");
+    if (s == 0 || chunk + n + 1 > most) first_seq.push_back(s), chunk = 0;
+    chunk += n + 1;
+    for (int i = 0; i <= n; ++i) t_pos.push_back(a + from - 1 + i);
+    for (int i = 0; i < n; ++i) d_pos.push_back(a + from - 1 + i), tok.push_back(tokens[a + from + i]);
+    off.push_back((int32_t)tok.size());
+  }
+  first_seq.push_back(n_seq);
+  const int n = (int)tok.size();
+  if (n > 0 && !u_accept) return c->fail(RT_ERR_BAD_ARG, "random numbers missing");
+  // both models' hidden states
+  for (rt_model* x : {m, draft}) {
+    if (!x) continue;
+    const std::vector<int32_t>& pos = x == m ? t_pos : d_pos;
+    const std::vector<int32_t> ttok(pos.size(), 0);
+    int M = 0;
+    x->staged_tokens = 0;
+    RT_TRY(upload_batch(x, tokens, seq_offsets, n_seq, pos.data(), ttok.data(), nullptr, (int)pos.size(), false, &M));
+    x->staged_tokens = M;
+    x->staged_targets = (int)pos.size();
+    x->staged_has_weights = false;
+    const HeadScope scope(x, rt_model::HEAD_NONE, 1.f, 0, 0, 0);
+    RT_TRY(run_staged(x, false, nullptr));
+  }
+  // one block each way: tokens, random numbers, a chunk's offsets (from 0 on) behind one another; accepted, token
+  std::vector<int32_t> block(tok);
+  auto put = [&](const void* p, size_t words) { const size_t at = block.size(); if (words) { block.resize(at + words); memcpy(block.data() + at, p, words * 4); } return at; };
+  const size_t o_ua = put(u_accept, (size_t)n), o_us = put(u_sample, (size_t)n_seq);
+  std::vector<size_t> o_off;
+  for (size_t i = 0; i + 1 < first_seq.size(); ++i) {
+    o_off.push_back(block.size());
+    for (int s = first_seq[i]; s <= first_seq[i + 1]; ++s) block.push_back(off[s] - off[first_seq[i]]);
+  }
+  const size_t o_res = block.size();
+  if (!m->drafts.reserve((o_res + 2 * (size_t)n_seq) * 4)) return c->fail(RT_ERR_CUDA, "out of device memory (drafts)");
+  int32_t* dev = m->drafts.as<int32_t>();
+  RT_CUDA(c, cudaMemcpyAsync(dev, block.data(), o_res * 4, cudaMemcpyHostToDevice, c->stream));
+  RT_CUDA(c, cudaStreamSynchronize(c->stream));  // `block` leaves scope with the call
+  const PdlScope pdl_scope((size_t)seq_offsets[n_seq]);
+  rt_linear head, draft_head;
+  head.ctx = draft_head.ctx = c;
+  head.w = m->lm_head;
+  if (draft) draft_head.w = draft->lm_head;
+  const int V = m->cfg.vocab;
+  for (size_t i = 0; i + 1 < first_seq.size(); ++i) {
+    const int s0 = first_seq[i], s1 = first_seq[i + 1], d0 = off[s0], nd = off[s1] - d0;
+    const VocabRows p{m->logits.p, RT_DT_F32, (size_t)V};
+    RT_TRY(head_logits(m, &head, d0 + s0, nd + s1 - s0));
+    if (launch_softmax_rows(c, p, nd + s1 - s0, V, temperature, m->logits.p, RT_DT_F32, V)) return c->fail(RT_ERR_CUDA, "softmax launch failed");
+    VocabRows q{nullptr, RT_DT_F32, (size_t)V};
+    if (draft && nd > 0) {
+      q.p = draft->logits.p;
+      RT_TRY(head_logits(draft, &draft_head, d0, nd));
+      if (launch_softmax_rows(c, q, nd, V, temperature, draft->logits.p, RT_DT_F32, V)) return c->fail(RT_ERR_CUDA, "softmax launch failed");
+    }
+    const VerifyArgs a{p, q, V, dev + d0, dev + o_off[i], s1 - s0, nd, (const float*)dev + o_ua + d0, (const float*)dev + o_us + s0, dev + o_res + s0,
+                       dev + o_res + n_seq + s0};
+    if (launch_verify_draft(c, a)) return c->fail(RT_ERR_CUDA, "verification launch failed");
+  }
+  for (rt_model* x : {m, draft})
+    if (x) x->staged_tokens = 0;
+  RT_CUDA(c, cudaMemcpyAsync(accepted_out, dev + o_res, (size_t)n_seq * 4, cudaMemcpyDeviceToHost, c->stream));
+  RT_CUDA(c, cudaMemcpyAsync(token_out, dev + o_res + n_seq, (size_t)n_seq * 4, cudaMemcpyDeviceToHost, c->stream));
+  return c->check_device_status("rt_model_verify_draft");
 }
 
 rt_status rt_optim_step(rt_model* m, float lr, float max_norm, float beta1, float beta2, float eps, float wd,

@@ -151,6 +151,19 @@ struct rt_model {
   DevBuf xs, ns16, logits, dl16, sc_l, dns, dxs;
   DevBuf argmax;            // per target, the greedy token of the last pass that asked for it
   bool want_argmax = false;
+  // What the head does with the logits of the target rows: scores them against their tokens (with gradients in a training pass), hands
+  // out the largest, learns from a teacher's, or nothing (verification comes to the rows afterwards).
+  enum HeadKind { HEAD_SCORE, HEAD_TOP, HEAD_DISTILL, HEAD_NONE };
+  struct HeadWork {
+    HeadKind kind = HEAD_SCORE;
+    float temperature = 1.f;
+    int k = 0, mode = 0;
+  } head;
+  DevBuf lists;             // of the targets: indices [n x k], then log-probabilities [n x k] (a teacher's, or what HEAD_TOP finds, then lse [n])
+  int list_targets = 0;     // n of them
+  int* list_index() const { return lists.as<int>(); }
+  float* list_logp() const { return lists.as<float>() + (size_t)list_targets * head.k; }
+  DevBuf drafts;            // of a verification: tokens, offsets, random numbers, results
   DevBuf refresh_tab;       // device copy of refresh_sent
   std::vector<rt::LoraRefreshJob> refresh_jobs, refresh_sent;
   // A batch travels as one block: laid out in pinned memory, one copy to `batch`, the pointers below into it

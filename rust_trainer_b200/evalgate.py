@@ -1,6 +1,6 @@
 """Forward-only scoring for the eval gate (reference src/eval.rs:156-221) on the device model:
 `greedy_prefix`, `greedy_prefix_batch` and the packing rule `worth_packing`, which the trainer
-consults too (src/train.rs:255)."""
+consults too (src/train.rs:255); and `accepted_prefix`, the same question with random numbers in the place of the argmax."""
 from __future__ import annotations
 
 import os
@@ -62,3 +62,17 @@ def greedy_prefix_batch(model, examples):
     pos = np.asarray(all_pos, dtype=np.int32)
     am = model.argmax_at_packed([p], pos) if p is not None else model.argmax_at([t for t, _ in exs], pos)
     return [(_prefix_len(am[a:b], t[start:start + (b - a)]), b - a) for (t, start), (a, b, _) in zip(exs, spans)]
+
+
+def accepted_prefix(model, examples, rng, temperature: float = 1.0, draft=None):
+    """The sampling counterpart of greedy_prefix_batch: per (tokens, answer_start) example, how long a prefix of the answer the
+    model lets stand as drafts of `draft` (None: as drafts without probabilities), the answer's length, and the token that it
+    puts behind that prefix.  `rng` (a NumPy generator) gives the random numbers.  No counterpart in the reference."""
+    exs = [(np.asarray(t, dtype=np.int32), max(int(a), 1)) for t, a in examples]
+    exs = [(t, min(a, t.size)) for t, a in exs]
+    if not exs:
+        return []
+    ua = rng.random(sum(t.size - a for t, a in exs), dtype=np.float32)
+    us = rng.random(len(exs), dtype=np.float32)
+    accepted, token = model.verify_draft([t for t, _ in exs], [a for _, a in exs], ua, us, temperature, draft)
+    return [(int(n), t.size - a, int(x)) for n, (t, a), x in zip(accepted, exs, token)]

@@ -10,6 +10,7 @@ import numpy as np
 from ._lib import ModelConfig, RtError, lib
 from .frozen import Context, _fp
 from .linear import Linear
+from .ops import distill_mode
 
 _I32P = C.POINTER(C.c_int32)
 
@@ -175,6 +176,55 @@ class Model:
         self.ctx.check(lib().rt_model_argmax_layout(self._h, _ip(toks), _ip(offs), len(groups), _ip(pos), _ip(seg), _ip(tp),
                                                     tp.size, _ip(out)))
         return out
+
+    def _targets(self, seqs, groups):
+        """tokens, offsets, number of sequences, positions, segments of plain sequences or packed groups."""
+        if (seqs is None) == (groups is None):
+            raise RtError(7, "either sequences or packed groups")
+        if groups is None:
+            toks, offs = self._batch(seqs)
+            return toks, offs, len(seqs), None, None
+        toks, offs, pos, seg = self._layout(groups)
+        return toks, offs, len(groups), pos, seg
+
+    def top_logits(self, seqs, target_pos, k: int, temperature: float = 1.0, groups=None):
+        """What a teacher hands on: the k largest logits at each (global) position of a forward-only pass, as (index
+        [n x k], log-probability [n x k], log-sum-exp [n]) at the temperature.  `groups` (with seqs None): packed groups."""
+        toks, offs, n_seq, pos, seg = self._targets(seqs, groups)
+        tp = np.ascontiguousarray(target_pos, dtype=np.int32)
+        index, logp, lse = np.empty((tp.size, max(k, 0)), np.int32), np.empty((tp.size, max(k, 0)), np.float32), np.empty(tp.size, np.float32)
+        self.ctx.check(lib().rt_model_top_logits(self._h, _ip(toks), _ip(offs), n_seq, None if pos is None else _ip(pos), None if seg is None else _ip(seg),
+                                                 _ip(tp), tp.size, temperature, k, _ip(index), _fp(logp), _fp(lse)))
+        return index, logp, lse
+
+    def distill_backward(self, seqs, target_pos, index, teacher_logp, weights, temperature: float = 1.0, mode: str = "renorm", groups=None) -> np.ndarray:
+        """Adds the gradient of the weighted divergence from a teacher's lists (index -1: no entry) into every adapter's
+        gradients; returns the weighted loss of each target."""
+        toks, offs, n_seq, pos, seg = self._targets(seqs, groups)
+        tp = np.ascontiguousarray(target_pos, dtype=np.int32)
+        index, t = np.ascontiguousarray(index, dtype=np.int32), np.ascontiguousarray(teacher_logp, dtype=np.float32)
+        w = np.ascontiguousarray(weights, dtype=np.float32)
+        if index.ndim != 2 or index.shape != t.shape or not (index.shape[0] == tp.size == w.size):
+            raise RtError(1, "targets, lists and weights differ in length")
+        loss = np.empty(tp.size, dtype=np.float32)
+        self.ctx.check(lib().rt_model_distill_backward(self._h, _ip(toks), _ip(offs), n_seq, None if pos is None else _ip(pos), None if seg is None else _ip(seg),
+                                                       _ip(tp), _fp(w), tp.size, temperature, distill_mode(mode), index.shape[1], _ip(index), _fp(t),
+                                                       _fp(loss)))
+        return loss
+
+    def verify_draft(self, seqs, draft_from, u_accept, u_sample, temperature: float = 1.0, draft: "Model | None" = None):
+        """Which of the tokens seqs[s][draft_from[s]:] this model lets stand against the random numbers, drafted by the model
+        `draft` (None: without probabilities): (accepted [n_seq], the token behind them [n_seq])."""
+        toks, offs = self._batch(seqs)
+        start = np.ascontiguousarray(draft_from, dtype=np.int32)
+        ua, us = np.ascontiguousarray(u_accept, dtype=np.float32), np.ascontiguousarray(u_sample, dtype=np.float32)
+        n = int((offs[1:] - offs[:-1] - start).sum()) if start.shape == (len(seqs),) else -1
+        if us.shape != (len(seqs),) or ua.size != n:
+            raise RtError(1, "a start and a number for each sequence, a number for each drafted token")
+        accepted, token = np.empty(len(seqs), np.int32), np.empty(len(seqs), np.int32)
+        self.ctx.check(lib().rt_model_verify_draft(self._h, None if draft is None else draft._h, _ip(toks), _ip(offs), len(seqs), _ip(start), temperature,
+                                                   _fp(ua), _fp(us), _ip(accepted), _ip(token)))
+        return accepted, token
 
     def allreduce_grads(self) -> None:
         """Sum of the flat LoRA-gradient buffer over the ranks of the context's communicator."""

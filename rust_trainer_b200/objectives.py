@@ -1,4 +1,4 @@
-"""The trainer's two objectives as batch calls on the device model.
+"""The trainer's two objectives, and distillation, as batch calls on the device model.
 
 Mirrors `Trainer::example_grad` (src/train.rs:269-297) and `ensure_ref_logps` (src/train.rs:229-246):
 the reference walks a batch one example at a time; gradients simply add over examples, so here a
@@ -10,6 +10,9 @@ whole batch is ONE `forward_backward` call with per-target weights.
   [chosen | rejected] with constant weights +c on the chosen targets, -c on the rejected ones,
   c = beta*sigmoid(-z)/batch_n  (dL/dpc = -c, dL/dpr = +c; `forward_backward` accumulates the
   gradient of -sum(w*logp), as the reference's does).
+* distillation (no counterpart in the reference): a teacher's top logits at the answer positions, from a larger model or from this
+  one with its adapters off, then one pass in which every answer target learns from its list with the weight
+  T^2/batch_tokens (softening by T shrinks the gradient by T^2).
 """
 from __future__ import annotations
 
@@ -89,3 +92,18 @@ def dpo_batch_grad(model, pairs, ref_logps, beta: float) -> float:
         w[a:b] = c
     model.forward_backward(seqs, tp, tt, w)
     return float(loss)
+
+
+def teacher_top_logits(teacher, examples, k: int, temperature: float = 1.0):
+    """The teacher's k largest logits at every answer target of the batch, one forward-only call: (index, log-probability)."""
+    seqs, tp, _, _ = _layout(examples)
+    index, logp, _ = teacher.top_logits(seqs, tp, k, temperature)
+    return index, logp
+
+
+def distill_batch_grad(model, examples, teacher_lists, temperature: float = 1.0, mode: str = "tail") -> float:
+    """Accumulates the distillation gradient of a batch of examples; returns its loss."""
+    seqs, tp, _, _ = _layout(examples)
+    index, logp = teacher_lists
+    w = np.full(tp.size, np.float32(temperature) ** 2 / np.float32(tp.size), np.float32)
+    return float(model.distill_backward(seqs, tp, index, logp, w, temperature, mode).sum(dtype=np.float32))
