@@ -19,8 +19,9 @@ __device__ __forceinline__ TopKey top_key(float v, int c) {
   return ((TopKey)order32(v) << TOP_INDEX_BITS) | (uint32_t)((1 << TOP_INDEX_BITS) - 1 - c);
 }
 
-struct alignas(8) TopStat {
-  float m, s;
+struct alignas(16) TopStat {
+  float R, s;  // the sum of the warp's exponentials is s 2^R
+  float m, unused;
 };
 
 // the lanes' values in descending order
@@ -38,25 +39,35 @@ __device__ __forceinline__ uint32_t warp_sort(uint32_t v) {
   return v;
 }
 
-// A running reference, and the sum of exponentials relative to it.  It changes when an element is 2^60 times as large, so rarely.
+// Sums of exponentials as 2^(x hi - R), hi = log2(e) / T in f32 and R an integer, so that the product and the difference are rounded once,
+// together, and sums with different R meet exactly.  What hi leaves out is another temperature by 2^-26 or so: the row's log-sum-exp makes up for it,
+// as far as the mass is near the row's maximum.  R is set by the first elements, and again when one is 2^60 times as large, so rarely.
+// Elements that are too large or too far down for such an R (beyond 2^22 in units of T / log2(e)) have none: R = inf, or stays -inf, and a
+// row that has no other is summed again, relative to its maximum.
 struct RunningSum {
-  float m = -INFINITY;
+  float R = -INFINITY, most = -INFINITY;  // most: elements up to here need no other R
   F2 s[2] = {0, 0};
-  __device__ __forceinline__ void take(const float (&x)[16], float largest, float most, const ExpT& ex) {
-    if (!(largest <= m + most) && m == m) {  // the first finite ones, ones that are far larger, a NaN, which stays
-      const float by = m > -INFINITY ? ex(m - largest) : 0.0f;
-      s[0] = mul2(s[0], pack2(by, by));
-      s[1] = mul2(s[1], pack2(by, by));
-      m = largest;
+  __device__ __forceinline__ void take(const float (&x)[16], float largest, float hi) {
+    if (!(largest <= most)) {
+      if (R == R) {  // a NaN stays
+        const float to = largest == largest ? ceilf(largest * hi) : NAN;
+        if (!(to < -4194304.0f)) {
+          const float by = R > -INFINITY ? ex2(R - to) : 0.0f;
+          s[0] = mul2(s[0], pack2(by, by));
+          s[1] = mul2(s[1], pack2(by, by));
+          R = to > 4194304.0f ? INFINITY : to;
+          most = (R + 60.0f) / hi;
+        }
+      }
     }
-    const float ref = m > -INFINITY ? m : 0.0f;
-    const F2 minus_ref = pack2(-ref, -ref);
+    const float r = R > -INFINITY ? -R : 0.0f;
+    const F2 minus_r = R > -INFINITY ? pack2(r, r) : pack2(-INFINITY, -INFINITY), by = pack2(hi, hi);
     F2 acc[2] = {0, 0};
 #pragma unroll
     for (int i = 0; i < 16; i += 2) {
       float a, b;
-      ex.pair(pack2(x[i], x[i + 1]), minus_ref, &a, &b);
-      acc[i / 2 & 1] = add2(acc[i / 2 & 1], pack2(a, b));
+      unpack2(fma2(pack2(x[i], x[i + 1]), by, minus_r), &a, &b);
+      acc[i / 2 & 1] = add2(acc[i / 2 & 1], pack2(ex2(a), ex2(b)));
     }
     s[0] = add2(s[0], acc[0]);
     s[1] = add2(s[1], acc[1]);
@@ -73,7 +84,7 @@ top_logits_kernel(const T* z, size_t ld, size_t rows, int vocab, float t, ExpT e
   __shared__ TopStat stats[2][VR_MAX_CLUSTER * WARPS];
   __shared__ uint2 told[2][VR_MAX_CLUSTER];  // what every CTA told
   __shared__ uint32_t sample[32 * SAMPLE_LANE];
-  __shared__ double s_log_sum;
+  __shared__ double s_lse, s_sums[WARPS];
   __shared__ int s_kept, s_n, s_count[2], s_found[VR_MAX_CLUSTER];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (tid == 0) s_kept = s_n = s_count[0] = s_count[1] = 0;
@@ -84,7 +95,7 @@ top_logits_kernel(const T* z, size_t ld, size_t rows, int vocab, float t, ExpT e
     return;
   }
   const double inv_t = 1.0 / t;
-  const float most = 60.0f / ex.hi;
+  const float hi = ex.hi;
   // values of a warp in the sample: W warps send at most W + k + W of them
   const int each = min((k + WARPS - 1) / WARPS + 1, 32), warps = ring.size * WARPS;
   TopKey *kept = (TopKey*)slots, *room = kept + TOP_KEPT;
@@ -137,68 +148,90 @@ top_logits_kernel(const T* z, size_t ld, size_t rows, int vocab, float t, ExpT e
       from = order32_value(b);
     };
     const int n_steps = (part.n_it + STEP - 1) / STEP;
+#pragma unroll 1
     for (int s = 0; s < n_steps; ++s) {
-      float x[16];
-      const int read = min((s + 1) * STEP, part.n_it) - s * STEP;
+      uint4 v[STEP];
+      const int read = min(STEP, part.n_it - s * STEP);
+      if (s > 0 && s + 1 < n_steps) {
 #pragma unroll
-      for (int j = 0; j < STEP; ++j) {
-        const int it = s * STEP + j;
-        if (j < read) {
-          ring.wait(it);
-          if (part.outer(it)) {
-            ring.complete(part, it);
-            fence_proxy_async_smem();  // what it wrote comes before the copies that follow
+        for (int j = 0; j < STEP; ++j) ring.wait(s * STEP + j);
+#pragma unroll
+        for (int j = 0; j < STEP; ++j) v[j] = ring.block(s * STEP + j)[tid];
+      } else {
+#pragma unroll
+        for (int j = 0; j < STEP; ++j) {
+          v[j] = make_uint4(Part::NONE, Part::NONE, Part::NONE, Part::NONE);
+          if (j >= read) continue;
+          ring.wait(s * STEP + j);
+          ring.complete(part, s * STEP + j);
+          v[j] = ring.block(s * STEP + j)[tid];
+        }
+        fence_proxy_async_smem();  // what was written there comes before the copies that follow
+      }
+      float x[16], top;
+#pragma unroll
+      for (int j = 0; j < STEP; ++j) Part::unpack(v[j], x + j * VEC);
+      if constexpr (sizeof(T) == 4) {
+        top = max_nan(x[0], x[1], x[2]);
+#pragma unroll
+        for (int i = 3; i < 15; i += 2) top = max_nan(top, x[i], x[i + 1]);
+        top = max_nan(top, x[15]);
+      } else {
+        using T2 = std::conditional_t<std::is_same<T, __half>::value, __half2, __nv_bfloat162>;
+        T2 m = __hmax2_nan(__hmax2_nan(*(const T2*)&v[0].x, *(const T2*)&v[0].y), __hmax2_nan(*(const T2*)&v[0].z, *(const T2*)&v[0].w));
+        m = __hmax2_nan(m, __hmax2_nan(__hmax2_nan(*(const T2*)&v[1].x, *(const T2*)&v[1].y), __hmax2_nan(*(const T2*)&v[1].z, *(const T2*)&v[1].w)));
+        top = max_nan(to_f32(m.x), to_f32(m.y));
+      }
+      sum.take(x, top, hi);
+      largest = max_nan(largest, top);
+      // for a bound: after 1, 4, 16 ... steps (1, 2, 4, 8 ... for long lists), but not shortly before the end
+      if ((s & (s + 1)) == 0 && (k > 64 || (s + 1) % 3 == 1) && (s == 0 || (s + 1) * 4 < n_steps * 3)) set_bound(bound_of(largest));
+      if (!(top < from)) {  // NaN too
+        uint32_t hits = 0;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) hits |= x[i] < from ? 0 : 1u << i;
+        if (*(volatile int*)&s_kept <= TOP_KEPT) {  // else there are too many already
+          int p = atomicAdd(&s_kept, __popc(hits));
+          for (; hits && p < TOP_KEPT; ++p, hits &= hits - 1) {
+            const int i = __ffs(hits) - 1, j = i / VEC, e = i % VEC, it = s * STEP + j, c = part.column(it) + e;
+            // what lies outside of the row is below every element
+            kept[p] = j < read && c >= 0 && c < vocab ? top_key(to_f32(((const T*)(ring.block(it) + tid))[e]), c) : 0;
           }
-          Part::unpack(ring.block(it)[tid], x + j * VEC);
-        } else {
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) x[j * VEC + i] = -INFINITY;
         }
       }
       __syncwarp();
       if (lane < read) mbar_arrive(ring.empty + ring.place(s * STEP + lane));
-      float top = max_nan(x[0], x[1], x[2]);
-#pragma unroll
-      for (int i = 3; i < 15; i += 2) top = max_nan(top, x[i], x[i + 1]);
-      top = max_nan(top, x[15]);
-      sum.take(x, top, most, ex);
-      largest = max_nan(largest, top);
-      // for a bound: after 1, 4, 16 ... steps (1, 2, 4, 8 ... for long lists), but not shortly before the end
-      if ((s & (s + 1)) == 0 && (k > 64 || (s + 1) % 3 == 1) && (s == 0 || (s + 1) * 4 < n_steps * 3)) {
-        set_bound(bound_of(largest));
-        if (*(volatile int*)&s_kept > TOP_KEPT) from = INFINITY;  // too many already: none any more
-      }
-      if (!(top < from)) {  // NaN too
-        if (*(volatile int*)&s_kept <= TOP_KEPT) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            if (x[i] < from) continue;
-            const int it = s * STEP + i / VEC, c = part.column(it) + i % VEC;
-            if (it >= part.n_it || c < 0 || c >= vocab) continue;
-            const int p = atomicAdd(&s_kept, 1);
-            if (p < TOP_KEPT) kept[p] = top_key(x[i], c);
-          }
-        }
-      }
       ring.advance(read, s + 1 == n_steps);
     }
     set_bound(bound_of(largest));
     TopStat st;
-    float a, b;
-    unpack2(add2(sum.s[0], sum.s[1]), &a, &b);
-    st.s = warp_join(sum.m, a + b, ex, &st.m);
+    {
+      float a, b;
+      unpack2(add2(sum.s[0], sum.s[1]), &a, &b);
+      st.R = warp_max_nan(sum.R);
+      st.m = warp_max_nan(largest);
+      st.s = warp_sum_f32(sum.R > -INFINITY ? (a + b) * ex2(sum.R - st.R) : 0.0f);
+    }
     TopStat* stat = stats[exchange.turn()];
     uint2* to = told[exchange.turn()];
     const int n_kept = s_kept;  // all have been counted before the bound's barriers
     if (tid == 0) exchange.expect(warps * sizeof(TopStat) + ring.size * 8);
-    if (lane < ring.size) send(mapa_u32(smem_u32(&stat[ring.rank * WARPS + warp]), lane), exchange.bar(lane), __float_as_uint(st.m), __float_as_uint(st.s));
+    if (lane < ring.size)
+      send(mapa_u32(smem_u32(&stat[ring.rank * WARPS + warp]), lane), exchange.bar(lane), __float_as_uint(st.R), __float_as_uint(st.s), __float_as_uint(st.m), 0u);
     if (tid < ring.size) send(mapa_u32(smem_u32(to + ring.rank), tid), exchange.bar(tid), bound, (uint32_t)n_kept);
     exchange.wait();
-    float m;
-    const double lane_sum = lane_join(warps, [&](int i, float* mi, float* si) { *mi = stat[i].m, *si = stat[i].s; }, ex, &m);
-    if (warp == WARPS - 1) {
-      const double all = warp_sum_f64(lane_sum);
-      if (lane == 0) s_log_sum = log(all);
+    float m = -INFINITY, R = -INFINITY;
+    for (int i = lane; i < warps; i += 32) m = max_nan(m, stat[i].m), R = max_nan(R, stat[i].R);
+    m = warp_max_nan(m);
+    R = warp_max_nan(R);
+    const bool bad = !(m < INFINITY), again = !bad && m > -INFINITY && !(R > -INFINITY && R < INFINITY);
+    if (warp == WARPS - 1 && !again) {
+      double all = 0.0;
+      for (int i = lane; i < warps; i += 32)
+        if (stat[i].R > -INFINITY) all += (double)(stat[i].s * ex2(stat[i].R - R));
+      all = warp_sum_f64(all);
+      // log sum 2^(x (hi + lo)), of which R and the sum have hi
+      if (lane == 0) s_lse = bad ? NAN : m == -INFINITY ? -INFINITY : log(all) + ((double)R + (double)m * ex.lo) * 0.69314718055994530942;
     }
     bool fits = true;
     for (int i = 0; i < ring.size; ++i) {  // every CTA's bound holds for the row
@@ -218,14 +251,30 @@ top_logits_kernel(const T* z, size_t ld, size_t rows, int vocab, float t, ExpT e
     work_sync<NT>();
     const uint2* found = tell((uint32_t)s_n, 0);
     for (int i = 0; i < ring.size; ++i) fits &= found[i].x <= (uint32_t)room_each;
-    if (!fits) {
-      auto each_element = [&](auto&& f) {
+    // the thread's elements once more, which is rare
+    auto each_element = [&](auto&& f) {
 #pragma unroll 1
-        for (int it = 0; it < part.n_it; ++it) {
-          const int c0 = part.column(it);
-          for (int c = max(c0, 0); c < min(c0 + VEC, vocab); ++c) f(to_f32(part.row[c]), c);
-        }
-      };
+      for (int it = 0; it < part.n_it; ++it) {
+        const int c0 = part.column(it);
+        for (int c = max(c0, 0); c < min(c0 + VEC, vocab); ++c) f(to_f32(part.row[c]), c);
+      }
+    };
+    if (again) {
+      double mine = 0.0;
+      each_element([&](float v, int) { mine += ex(v - m); });
+      mine = warp_sum_f64(mine);
+      if (lane == 0) s_sums[warp] = mine;
+      work_sync<NT>();
+      double all = 0.0;  // of the CTA's elements, and of the cluster's
+      for (int i = 0; i < WARPS; ++i) all += s_sums[i];
+      const uint2* sums = tell(__double2loint(all), __double2hiint(all));
+      all = 0.0;
+      for (int i = 0; i < ring.size; ++i) all += __hiloint2double(sums[i].y, sums[i].x);
+      work_sync<NT>();
+      if (tid == 0) s_lse = log(all) + (double)m * inv_t;
+      work_sync<NT>();
+    }
+    if (!fits) {
       // elements that are at least `key`, in all, and whether every CTA's have room
       int round = 0;
       auto count = [&](TopKey key, bool* room_for_all) {
@@ -278,9 +327,8 @@ top_logits_kernel(const T* z, size_t ld, size_t rows, int vocab, float t, ExpT e
       }
       exchange.wait();
     }
-    const bool bad = !(m < INFINITY);
-    const double log_sum = s_log_sum;
-    if (lse && tid == 0 && ring.rank == 0) lse[r] = bad ? NAN : (float)(m * inv_t + log_sum);
+    const double row_lse = s_lse;
+    if (lse && tid == 0 && ring.rank == 0) lse[r] = (float)row_lse;
     // a warp an element: its rank is the number of larger ones
     for (int i = warp; i < n_mine; i += WARPS) {
       const TopKey key = mine[i];
@@ -293,7 +341,7 @@ top_logits_kernel(const T* z, size_t ld, size_t rows, int vocab, float t, ExpT e
       if (rank >= k || lane > 0) continue;
       const float v = order32_value((uint32_t)(key >> TOP_INDEX_BITS));
       index[r * k + rank] = (1 << TOP_INDEX_BITS) - 1 - (int)(key & ((1 << TOP_INDEX_BITS) - 1));
-      logp[r * k + rank] = bad ? NAN : v == -INFINITY ? -INFINITY : (float)(((double)v - m) * inv_t - log_sum);
+      logp[r * k + rank] = bad ? NAN : v == -INFINITY ? -INFINITY : (float)(v * inv_t - row_lse);
     }
     work_sync<NT>();
     if (tid == 0) s_n = s_kept = 0;  // the next row's first bound has barriers before they count again
