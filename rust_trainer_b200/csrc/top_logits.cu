@@ -9,8 +9,13 @@
 
 namespace rt {
 
-constexpr int TOP_KEPT = 3072, TOP_ROOM = 2048;  // elements that are kept on the way, and that are ranked, at most
-static_assert(TOP_ROOM / VR_MAX_CLUSTER >= RT_TOP_MAX, "k elements of one CTA's share have to fit");
+// Elements that are kept on the way, and that are ranked, at most: in proportion to what random rows need, some 12 k and 2 k.
+struct TopRoom {
+  int kept, ranked;
+};
+constexpr int TOP_SHORT = 64;  // entries of a list that 256 threads make
+static TopRoom top_room(int k, int cluster) { return k <= TOP_SHORT ? TopRoom{1536, cluster == 1 ? 768 : 256 * cluster} : TopRoom{3584, cluster == 1 ? 1024 : 256 * cluster}; }
+static_assert(RT_TOP_MAX <= 256, "k elements of one CTA's share have to fit");
 // An element as an integer, all different: its value's order above, the lower index in front.
 constexpr int TOP_INDEX_BITS = 19;
 static_assert(RT_VOCAB_MAX <= 1 << TOP_INDEX_BITS);
@@ -74,11 +79,68 @@ struct RunningSum {
   }
 };
 
+// The row as it streams by: units of 16 elements a thread, dealt to the cluster's CTAs in turn, each one bulk copy into a ring (what
+// vocab_rows.cuh's is in blocks, where rows stay).
+template <class T, int NT>
+struct UnitRing {
+  static constexpr int VEC = 16 / (int)sizeof(T), STEP = 16 / VEC, UNIT = STEP * NT;  // elements of a vector; vectors of a thread and of a unit
+  uint4* slots;            // [places][UNIT]
+  uint64_t *full, *empty;  // [places]
+  int* status;
+  int places, vocab, rank, size;
+  int place = 0;  // of the unit that comes next, and its phase
+  uint32_t phase = 0;
+  // of the row that is worked on
+  const T* row;
+  int align, n_vec, n_units;
+
+  __device__ __forceinline__ UnitRing(uint4* slots_, uint64_t* bars, int places_, int* status_, int vocab_, Exchange& exchange)
+      : slots(slots_), full(bars), empty(bars + VR_MAX_BLOCKS), status(status_), places(places_), vocab(vocab_), rank((int)cluster_ctarank()),
+        size((int)cluster_size()) {
+    exchange.bars = bars + 2 * VR_MAX_BLOCKS;
+    exchange.status = status;
+    for (int i = threadIdx.x; i < places; i += NT) {
+      mbar_init(full + i, 1);
+      mbar_init(empty + i, NT / 32);
+    }
+    if (threadIdx.x < 2) mbar_init(exchange.bars + threadIdx.x, 1);
+    mbar_fence_init();
+    fence_proxy_async_smem();
+    cluster_sync_all();  // nobody sends to a CTA that does not run yet
+  }
+  __device__ __forceinline__ void begin(const T* row_) {
+    row = row_;
+    align = (int)(((uintptr_t)row & 15) / sizeof(T));
+    n_vec = (align + vocab + VEC - 1) / VEC;
+    const int units = (n_vec + UNIT - 1) / UNIT;
+    n_units = (int)((unsigned)(units - rank + size - 1) / (unsigned)size);
+  }
+  __device__ __forceinline__ int first_vector(int s) const { return (s * size + rank) * UNIT; }
+  // the column of the first element of the thread's j-th vector of a unit
+  __device__ __forceinline__ int column(int s, int j) const { return (first_vector(s) + j * NT + (int)threadIdx.x) * VEC - align; }
+  __device__ __forceinline__ void next() {
+    if (++place == places) place = 0, phase ^= 1;
+  }
+  __device__ __forceinline__ void copy_rows(const T* z, size_t ld, size_t rows, size_t row_step) {
+    for (size_t r = cluster_id(); r < rows; r += row_step) {
+      begin(z + r * ld);
+      for (int s = 0; s < n_units; ++s, next()) {
+        const int first = first_vector(s), v0 = max(first, align ? 1 : 0), v1 = min(first + UNIT, (align + vocab) / VEC);  // vectors that lie in the row
+        const uint32_t bytes = v1 > v0 ? (uint32_t)(v1 - v0) * 16 : 0;
+        row_wait(empty + place, phase ^ 1, status);
+        mbar_expect_tx(full + place, bytes);
+        if (bytes) bulk_load_1d(slots + place * UNIT + (v0 - first), row + (v0 * VEC - align), bytes, full + place);
+      }
+    }
+  }
+};
+
 template <class T, int NT>
 __global__ void __launch_bounds__(NT + 32, ctas_of(NT))
-top_logits_kernel(const T* z, size_t ld, size_t rows, int vocab, float t, ExpT ex, int k, int* index, float* logp, float* lse, int places, int* status) {
-  using Part = RowPart<T, NT>;
-  constexpr int VEC = Part::VEC, STEP = Part::STEP, WARPS = NT / 32, SAMPLE_LANE = (RT_TOP_MAX + 2 * WARPS + 31) / 32;
+top_logits_kernel(const T* z, size_t ld, size_t rows, int vocab, float t, ExpT ex, int k, int* index, float* logp, float* lse, int places,
+                  int kept_most, int room_most, int* status) {
+  using Ring = UnitRing<T, NT>;
+  constexpr int VEC = Ring::VEC, STEP = Ring::STEP, WARPS = NT / 32, SAMPLE_LANE = ((NT == 256 ? TOP_SHORT : RT_TOP_MAX) + 2 * WARPS + 31) / 32;
   extern __shared__ uint4 slots[];
   __shared__ uint64_t bars[2 * VR_MAX_BLOCKS + 2];
   __shared__ TopStat stats[2][VR_MAX_CLUSTER * WARPS];
@@ -89,17 +151,18 @@ top_logits_kernel(const T* z, size_t ld, size_t rows, int vocab, float t, ExpT e
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (tid == 0) s_kept = s_n = s_count[0] = s_count[1] = 0;
   Exchange exchange;
-  Ring<T, NT> ring(slots + (TOP_KEPT + TOP_ROOM) / 2, bars, places, status, z, ld, rows, vocab, exchange);
+  Ring ring(slots + (kept_most + room_most) / 2, bars, places, status, vocab, exchange);
+  const size_t row_step = gridDim.x / (unsigned)ring.size;
   if (tid >= NT) {
-    if (tid == NT) ring.copy_rows();
+    if (tid == NT) ring.copy_rows(z, ld, rows, row_step);
     return;
   }
   const double inv_t = 1.0 / t;
   const float hi = ex.hi;
   // values of a warp in the sample: W warps send at most W + k + W of them
   const int each = min((k + WARPS - 1) / WARPS + 1, 32), warps = ring.size * WARPS;
-  TopKey *kept = (TopKey*)slots, *room = kept + TOP_KEPT;
-  const int room_each = TOP_ROOM / ring.size;
+  TopKey *kept = (TopKey*)slots, *room = kept + kept_most;
+  const int room_each = room_most / ring.size;
   // A value that k of the threads' maxima reach, and not many more of the sample's, in every warp the same.
   auto bound_of = [&](float largest) {
     const uint32_t sorted = warp_sort(order32(largest));
@@ -137,71 +200,89 @@ top_logits_kernel(const T* z, size_t ld, size_t rows, int vocab, float t, ExpT e
     exchange.wait();
     return (const uint2*)to;
   };
-  for (size_t r = cluster_id(); r < rows; r += ring.row_step) {
-    const Part part = ring.part(r);
+  for (size_t r = cluster_id(); r < rows; r += row_step) {
+    ring.begin(z + r * ld);
     RunningSum sum;
     float largest = -INFINITY;  // of the thread's elements
-    uint32_t bound = 0xffffffffu;
-    float from = NAN;
+    uint32_t bound = 0;
+    float from = 0.0f;  // elements from here up are kept
     auto set_bound = [&](uint32_t b) {
       bound = b;
       from = order32_value(b);
+      if (from == 0.0f) from = -1.4e-45f;  // the two zeros are equal, which the sign of a difference is not
     };
-    const int n_steps = (part.n_it + STEP - 1) / STEP;
 #pragma unroll 1
-    for (int s = 0; s < n_steps; ++s) {
-      uint4 v[STEP];
-      const int read = min(STEP, part.n_it - s * STEP);
-      if (s > 0 && s + 1 < n_steps) {
-#pragma unroll
-        for (int j = 0; j < STEP; ++j) ring.wait(s * STEP + j);
-#pragma unroll
-        for (int j = 0; j < STEP; ++j) v[j] = ring.block(s * STEP + j)[tid];
-      } else {
-#pragma unroll
+    for (int s = 0; s < ring.n_units; ++s) {
+      uint4* const at = ring.slots + ring.place * Ring::UNIT + tid;
+      row_wait(ring.full + ring.place, ring.phase, status);
+      if (s == 0 || s + 1 == ring.n_units) {
+        // what no copy brings: vectors that stick out of the row, element by element, and -inf behind its last one
+#pragma unroll 1
         for (int j = 0; j < STEP; ++j) {
-          v[j] = make_uint4(Part::NONE, Part::NONE, Part::NONE, Part::NONE);
-          if (j >= read) continue;
-          ring.wait(s * STEP + j);
-          ring.complete(part, s * STEP + j);
-          v[j] = ring.block(s * STEP + j)[tid];
+          const int c = ring.column(s, j);
+          if (c >= 0 && c + VEC <= vocab) continue;
+          alignas(16) T e[VEC];
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) e[i] = c + i >= 0 && c + i < vocab ? ring.row[c + i] : from_f32<T>(-INFINITY);
+          at[j * NT] = *(const uint4*)e;
         }
-        fence_proxy_async_smem();  // what was written there comes before the copies that follow
+        fence_proxy_async_smem();  // it comes before the copies that follow
       }
+      uint4 v[STEP];
+#pragma unroll
+      for (int j = 0; j < STEP; ++j) v[j] = at[j * NT];
       float x[16], top;
 #pragma unroll
-      for (int j = 0; j < STEP; ++j) Part::unpack(v[j], x + j * VEC);
+      for (int j = 0; j < STEP; ++j) unpack_vector<T>(v[j], x + j * VEC);
+      using T2 = std::conditional_t<std::is_same<T, __half>::value, __half2, __nv_bfloat162>;
+      const T2* const x2 = (const T2*)v;  // 16-bit elements in pairs
       if constexpr (sizeof(T) == 4) {
         top = max_nan(x[0], x[1], x[2]);
 #pragma unroll
         for (int i = 3; i < 15; i += 2) top = max_nan(top, x[i], x[i + 1]);
         top = max_nan(top, x[15]);
       } else {
-        using T2 = std::conditional_t<std::is_same<T, __half>::value, __half2, __nv_bfloat162>;
-        T2 m = __hmax2_nan(__hmax2_nan(*(const T2*)&v[0].x, *(const T2*)&v[0].y), __hmax2_nan(*(const T2*)&v[0].z, *(const T2*)&v[0].w));
-        m = __hmax2_nan(m, __hmax2_nan(__hmax2_nan(*(const T2*)&v[1].x, *(const T2*)&v[1].y), __hmax2_nan(*(const T2*)&v[1].z, *(const T2*)&v[1].w)));
+        T2 m = x2[0];
+#pragma unroll
+        for (int i = 1; i < 8; ++i) m = __hmax2_nan(m, x2[i]);
         top = max_nan(to_f32(m.x), to_f32(m.y));
       }
       sum.take(x, top, hi);
       largest = max_nan(largest, top);
-      // for a bound: after 1, 4, 16 ... steps (1, 2, 4, 8 ... for long lists), but not shortly before the end
-      if ((s & (s + 1)) == 0 && (k > 64 || (s + 1) % 3 == 1) && (s == 0 || (s + 1) * 4 < n_steps * 3)) set_bound(bound_of(largest));
+      // for a bound: after 1, 4, 16 ... units (1, 2, 4, 8 ... for long lists), but not shortly before the end
+      if ((s & (s + 1)) == 0 && (k > TOP_SHORT || (s + 1) % 3 == 1) && (s == 0 || (s + 1) * 4 < ring.n_units * 3)) set_bound(bound_of(largest));
       if (!(top < from)) {  // NaN too
+        // a bit for each element that is not below
         uint32_t hits = 0;
+        if constexpr (sizeof(T) == 4) {
+          const F2 minus_from = pack2(-from, -from);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) hits |= x[i] < from ? 0 : 1u << i;
-        if (*(volatile int*)&s_kept <= TOP_KEPT) {  // else there are too many already
+          for (int i = 0; i < 16; i += 2) {
+            float a, b;
+            unpack2(add2(pack2(x[i], x[i + 1]), minus_from), &a, &b);
+            hits = __funnelshift_l(__float_as_uint(a), hits, 1);
+            hits = __funnelshift_l(__float_as_uint(b), hits, 1);
+          }
+          hits = ~hits & 0xffff;
+        } else {
+          const T f = from_f32<T>(from == -1.4e-45f ? 0.0f : from);  // one of the elements, or a zero
+          T2 f2;
+          f2.x = f2.y = f;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) hits |= (~__hlt2_mask(x2[i], f2) & 0x00010001u) << i;
+        }
+        if (*(volatile int*)&s_kept <= kept_most) {  // else there are too many already
           int p = atomicAdd(&s_kept, __popc(hits));
-          for (; hits && p < TOP_KEPT; ++p, hits &= hits - 1) {
-            const int i = __ffs(hits) - 1, j = i / VEC, e = i % VEC, it = s * STEP + j, c = part.column(it) + e;
+          for (; hits && p < kept_most; ++p, hits &= hits - 1) {
+            const int bit = __ffs(hits) - 1, i = sizeof(T) == 4 ? 15 - bit : 2 * (bit & 15) + (bit >> 4), j = i / VEC, c = ring.column(s, j) + i % VEC;
             // what lies outside of the row is below every element
-            kept[p] = j < read && c >= 0 && c < vocab ? top_key(to_f32(((const T*)(ring.block(it) + tid))[e]), c) : 0;
+            kept[p] = c >= 0 && c < vocab ? top_key(to_f32(((const T*)(at + j * NT))[i % VEC]), c) : 0;
           }
         }
       }
       __syncwarp();
-      if (lane < read) mbar_arrive(ring.empty + ring.place(s * STEP + lane));
-      ring.advance(read, s + 1 == n_steps);
+      if (lane == 0) mbar_arrive(ring.empty + ring.place);
+      ring.next();
     }
     set_bound(bound_of(largest));
     TopStat st;
@@ -235,7 +316,7 @@ top_logits_kernel(const T* z, size_t ld, size_t rows, int vocab, float t, ExpT e
     }
     bool fits = true;
     for (int i = 0; i < ring.size; ++i) {  // every CTA's bound holds for the row
-      fits &= to[i].y <= (uint32_t)TOP_KEPT;
+      fits &= to[i].y <= (uint32_t)kept_most;
       bound = max(bound, to[i].x);
     }
     // elements to be ranked: this CTA's lie in its share of the room
@@ -254,9 +335,9 @@ top_logits_kernel(const T* z, size_t ld, size_t rows, int vocab, float t, ExpT e
     // the thread's elements once more, which is rare
     auto each_element = [&](auto&& f) {
 #pragma unroll 1
-      for (int it = 0; it < part.n_it; ++it) {
-        const int c0 = part.column(it);
-        for (int c = max(c0, 0); c < min(c0 + VEC, vocab); ++c) f(to_f32(part.row[c]), c);
+      for (int i = 0; i < ring.n_units * STEP; ++i) {
+        const int c0 = ring.column(i / STEP, i % STEP);
+        for (int c = max(c0, 0); c < min(c0 + VEC, vocab); ++c) f(to_f32(ring.row[c]), c);
       }
     };
     if (again) {
@@ -329,16 +410,17 @@ top_logits_kernel(const T* z, size_t ld, size_t rows, int vocab, float t, ExpT e
     }
     const double row_lse = s_lse;
     if (lse && tid == 0 && ring.rank == 0) lse[r] = (float)row_lse;
-    // a warp an element: its rank is the number of larger ones
-    for (int i = warp; i < n_mine; i += WARPS) {
+    // a thread an element: its rank is the number of larger ones
+    for (int i = tid; i < n_mine; i += NT) {
       const TopKey key = mine[i];
       int rank = 0;
       for (int o = 0; o < ring.size; ++o) {
         const int n = ring.size > 1 ? s_found[o] : n_mine;
-        for (int j = lane; j < n; j += 32) rank += room[o * room_each + j] > key;
+        const TopKey* const others = room + o * room_each;
+#pragma unroll 8
+        for (int j = 0; j < n; ++j) rank += others[j] > key;
       }
-      rank = __reduce_add_sync(0xffffffffu, rank);
-      if (rank >= k || lane > 0) continue;
+      if (rank >= k) continue;
       const float v = order32_value((uint32_t)(key >> TOP_INDEX_BITS));
       index[r * k + rank] = (1 << TOP_INDEX_BITS) - 1 - (int)(key & ((1 << TOP_INDEX_BITS) - 1));
       logp[r * k + rank] = bad ? NAN : v == -INFINITY ? -INFINITY : (float)(v * inv_t - row_lse);
@@ -349,13 +431,19 @@ top_logits_kernel(const T* z, size_t ld, size_t rows, int vocab, float t, ExpT e
 }
 
 int launch_top_logits(rt_ctx* c, const VocabRows& z, size_t rows, int vocab, float temperature, int k, int* index, float* logp, float* lse) {
-  // long lists want more threads, whose maxima are the sample that the bound is found in
-  const RowShape shape = stream_shape(c, rows, vocab, z.dtype, k <= 64 ? 256 : 512, (TOP_KEPT + TOP_ROOM) * sizeof(TopKey));
+  // Long lists want more threads, whose maxima are the sample that the bound is found in.  Three CTAs on an SM, or one; more CTAs a row
+  // where there are few rows.
+  const int threads = k <= TOP_SHORT ? 256 : 512, vec = z.dtype == RT_DT_F32 ? 4 : 8, units = (vec - 1 + vocab + 16 * threads - 1) / (16 * threads);
+  int size = 1;
+  while (size * 2 <= VR_MAX_CLUSTER && units > size && rows * size * 2 <= (size_t)c->num_sms) size *= 2;
+  const TopRoom room = top_room(k, size);
+  const size_t other = (room.kept + room.ranked) * sizeof(TopKey), unit = (size_t)threads * 16 * (z.dtype == RT_DT_F32 ? 4 : 2);
+  const int places = (int)std::min(((threads == 256 ? 70 : 208) * 1024 - other) / unit, (size_t)VR_MAX_BLOCKS);
   return with_dtype(z.dtype, [&](auto* zt) {
-    return with_threads(shape.threads, [&](auto threads) {
+    return with_threads(threads, [&](auto n) {
       using T = std::remove_pointer_t<decltype(zt)>;
-      return launch_clusters(c, top_logits_kernel<T, decltype(threads)::value>, true, rows, shape.threads + 32, shape.cluster, shape.smem, (const T*)z.p, z.ld,
-                             rows, vocab, temperature, exp_t(temperature), k, index, logp, lse, shape.places, c->status_dev);
+      return launch_clusters(c, top_logits_kernel<T, decltype(n)::value>, true, rows, threads + 32, size, places * unit + other, (const T*)z.p, z.ld, rows, vocab,
+                             temperature, exp_t(temperature), k, index, logp, lse, places, room.kept, room.ranked, c->status_dev);
     });
   });
 }

@@ -167,18 +167,31 @@ __device__ __forceinline__ bool work_sync_or(bool v) {
       : "memory");
   return r != 0;
 }
+// Waits for a phase of a barrier, asleep for up to some microseconds at a time: a warp that polls takes instructions from those that work.
 // The matmul's wait gives up when another kernel has reported anything; here an index out of range in one row must not end the
 // others' waits, so that only the time limit does.
-static __device__ __noinline__ void row_wait_slow(uint64_t* bar, uint32_t parity, int* status) {
+__device__ __forceinline__ uint32_t mbar_sleep(uint64_t* bar, uint32_t phase) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(phase), "r"(20000u)
+      : "memory");
+  return ok;
+}
+static __device__ __noinline__ void row_wait_slow(uint64_t* bar, uint32_t phase, int* status) {
   const long long t0 = clock64();
-  for (;;) {
-    for (int i = 0; i < 256; ++i)
-      if (mbar_try_wait(bar, parity)) return;
+  while (!mbar_sleep(bar, phase)) {
     if (clock64() - t0 > MBAR_WAIT_LIMIT_CYCLES) {
       report_status(status, SITE_VOCAB_ROW);
       return;
     }
   }
+}
+__device__ __forceinline__ void row_wait(uint64_t* bar, uint32_t phase, int* status) {
+  if (!mbar_sleep(bar, phase)) row_wait_slow(bar, phase, status);
 }
 
 // Where a row's elements are: its vectors, and the blocks of them that are this CTA's.
@@ -242,10 +255,6 @@ __device__ __forceinline__ void put_elements(O* out, int c, int vocab, const flo
 #pragma unroll
   for (int i = 0; i < VEC; ++i)
     if (c + i >= 0 && c + i < vocab) out[c + i] = from_f32<O>(x[i]);
-}
-
-__device__ __forceinline__ void row_wait(uint64_t* bar, uint32_t phase, int* status) {
-  if (!mbar_try_wait(bar, phase)) row_wait_slow(bar, phase, status);
 }
 
 // Values that go round the cluster: everybody sends to everybody, and waits until all of it has come.  Two barriers in turn (and two places for
@@ -545,15 +554,6 @@ inline RowShape row_shape(const rt_ctx* c, size_t rows, int vocab, int dtype, si
   const size_t block = (size_t)threads * 16, room = need(threads) <= third ? third : need(threads) <= half ? half : all;
   const size_t turns = (rows * size + c->num_sms - 1) / c->num_sms, each = (need(threads) - other) / block;
   const size_t places = std::max(each, std::min(std::min((room - other) / block, (size_t)VR_MAX_BLOCKS), each * std::min(turns, (size_t)4)));
-  return {threads, size, (int)places, places * block + other};
-}
-// The same for rows that stream by: a CTA a row, more where there are few rows; three CTAs on an SM.
-inline RowShape stream_shape(const rt_ctx* c, size_t rows, int vocab, int dtype, int threads, size_t other) {
-  const int vec = dtype == RT_DT_F32 ? 4 : 8, vectors = (vec - 1 + vocab + vec - 1) / vec;
-  const size_t block = (size_t)threads * 16, third = (threads == 256 ? 70 : 208) * 1024;
-  int size = 1;
-  while (size * 2 <= VR_MAX_CLUSTER && vectors > 512 * size && rows * size * 2 <= (size_t)c->num_sms) size *= 2;
-  const size_t places = std::min((third - other) / block, (size_t)VR_MAX_BLOCKS);
   return {threads, size, (int)places, places * block + other};
 }
 // Calls f with the number of threads that work as a constant.
