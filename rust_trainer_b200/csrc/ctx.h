@@ -53,7 +53,7 @@ struct rt_ctx {
     smem_raised.insert(fn);
     return true;
   }
-  // clusters that the device runs at once, by kernel, cluster size and shared memory (vocab_rows.cuh)
+  // clusters that the device runs at once, by kernel, cluster size and threads, and shared memory (vocab_rows.cuh)
   std::map<std::tuple<const void*, int, size_t>, int> clusters_at_once;
   // Waits for the stream and reads the page-locked status word; maps non-zero to an error and clears it and the device's.
   rt_status check_device_status(const char* where);

@@ -79,70 +79,15 @@ struct RunningSum {
   }
 };
 
-// The row as it streams by: units of 16 elements a thread, dealt to the cluster's CTAs in turn, each one bulk copy into a ring (what
-// vocab_rows.cuh's is in blocks, where rows stay).
-template <class T, int NT>
-struct UnitRing {
-  static constexpr int VEC = 16 / (int)sizeof(T), STEP = 16 / VEC, UNIT = STEP * NT;  // elements of a vector; vectors of a thread and of a unit
-  uint4* slots;            // [places][UNIT]
-  uint64_t *full, *empty;  // [places]
-  int* status;
-  int places, vocab, rank, size;
-  int place = 0;  // of the unit that comes next, and its phase
-  uint32_t phase = 0;
-  // of the row that is worked on
-  const T* row;
-  int align, n_vec, n_units;
-
-  __device__ __forceinline__ UnitRing(uint4* slots_, uint64_t* bars, int places_, int* status_, int vocab_, Exchange& exchange)
-      : slots(slots_), full(bars), empty(bars + VR_MAX_BLOCKS), status(status_), places(places_), vocab(vocab_), rank((int)cluster_ctarank()),
-        size((int)cluster_size()) {
-    exchange.bars = bars + 2 * VR_MAX_BLOCKS;
-    exchange.status = status;
-    for (int i = threadIdx.x; i < places; i += NT) {
-      mbar_init(full + i, 1);
-      mbar_init(empty + i, NT / 32);
-    }
-    if (threadIdx.x < 2) mbar_init(exchange.bars + threadIdx.x, 1);
-    mbar_fence_init();
-    fence_proxy_async_smem();
-    cluster_sync_all();  // nobody sends to a CTA that does not run yet
-  }
-  __device__ __forceinline__ void begin(const T* row_) {
-    row = row_;
-    align = (int)(((uintptr_t)row & 15) / sizeof(T));
-    n_vec = (align + vocab + VEC - 1) / VEC;
-    const int units = (n_vec + UNIT - 1) / UNIT;
-    n_units = (int)((unsigned)(units - rank + size - 1) / (unsigned)size);
-  }
-  __device__ __forceinline__ int first_vector(int s) const { return (s * size + rank) * UNIT; }
-  // the column of the first element of the thread's j-th vector of a unit
-  __device__ __forceinline__ int column(int s, int j) const { return (first_vector(s) + j * NT + (int)threadIdx.x) * VEC - align; }
-  __device__ __forceinline__ void next() {
-    if (++place == places) place = 0, phase ^= 1;
-  }
-  __device__ __forceinline__ void copy_rows(const T* z, size_t ld, size_t rows, size_t row_step) {
-    for (size_t r = cluster_id(); r < rows; r += row_step) {
-      begin(z + r * ld);
-      for (int s = 0; s < n_units; ++s, next()) {
-        const int first = first_vector(s), v0 = max(first, align ? 1 : 0), v1 = min(first + UNIT, (align + vocab) / VEC);  // vectors that lie in the row
-        const uint32_t bytes = v1 > v0 ? (uint32_t)(v1 - v0) * 16 : 0;
-        row_wait(empty + place, phase ^ 1, status);
-        mbar_expect_tx(full + place, bytes);
-        if (bytes) bulk_load_1d(slots + place * UNIT + (v0 - first), row + (v0 * VEC - align), bytes, full + place);
-      }
-    }
-  }
-};
-
 template <class T, int NT>
 __global__ void __launch_bounds__(NT + 32, ctas_of(NT))
 top_logits_kernel(const T* z, size_t ld, size_t rows, int vocab, float t, ExpT ex, int k, int* index, float* logp, float* lse, int places,
                   int kept_most, int room_most, int* status) {
-  using Ring = UnitRing<T, NT>;
-  constexpr int VEC = Ring::VEC, STEP = Ring::STEP, WARPS = NT / 32, SAMPLE_LANE = ((NT == 256 ? TOP_SHORT : RT_TOP_MAX) + 2 * WARPS + 31) / 32;
+  constexpr int STEP = sizeof(T) == 4 ? 4 : 2;
+  using Ring = UnitRing<T, NT, STEP>;
+  constexpr int VEC = Ring::VEC, WARPS = NT / 32, SAMPLE_LANE = ((NT == 256 ? TOP_SHORT : RT_TOP_MAX) + 2 * WARPS + 31) / 32;
   extern __shared__ uint4 slots[];
-  __shared__ uint64_t bars[2 * VR_MAX_BLOCKS + 2];
+  __shared__ uint64_t bars[2 * VR_MAX_UNITS + 2];
   __shared__ TopStat stats[2][VR_MAX_CLUSTER * WARPS];
   __shared__ uint2 told[2][VR_MAX_CLUSTER];  // what every CTA told
   __shared__ uint32_t sample[32 * SAMPLE_LANE];
@@ -151,7 +96,9 @@ top_logits_kernel(const T* z, size_t ld, size_t rows, int vocab, float t, ExpT e
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (tid == 0) s_kept = s_n = s_count[0] = s_count[1] = 0;
   Exchange exchange;
-  Ring ring(slots + (kept_most + room_most) / 2, bars, places, status, vocab, exchange);
+  Ring ring(slots + (kept_most + room_most) / 2, bars, places, status, vocab);
+  exchange.begin(bars + 2 * VR_MAX_UNITS, status);
+  cluster_sync_all();  // nobody sends to a CTA that does not run yet
   const size_t row_step = gridDim.x / (unsigned)ring.size;
   if (tid >= NT) {
     if (tid == NT) ring.copy_rows(z, ld, rows, row_step);
@@ -216,17 +163,8 @@ top_logits_kernel(const T* z, size_t ld, size_t rows, int vocab, float t, ExpT e
       uint4* const at = ring.slots + ring.place * Ring::UNIT + tid;
       row_wait(ring.full + ring.place, ring.phase, status);
       if (s == 0 || s + 1 == ring.n_units) {
-        // what no copy brings: vectors that stick out of the row, element by element, and -inf behind its last one
-#pragma unroll 1
-        for (int j = 0; j < STEP; ++j) {
-          const int c = ring.column(s, j);
-          if (c >= 0 && c + VEC <= vocab) continue;
-          alignas(16) T e[VEC];
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) e[i] = c + i >= 0 && c + i < vocab ? ring.row[c + i] : from_f32<T>(-INFINITY);
-          at[j * NT] = *(const uint4*)e;
-        }
-        fence_proxy_async_smem();  // it comes before the copies that follow
+        ring.complete(s, at);
+        fence_proxy_async_smem();  // what it wrote comes before the copies that follow
       }
       uint4 v[STEP];
 #pragma unroll
@@ -438,7 +376,7 @@ int launch_top_logits(rt_ctx* c, const VocabRows& z, size_t rows, int vocab, flo
   while (size * 2 <= VR_MAX_CLUSTER && units > size && rows * size * 2 <= (size_t)c->num_sms) size *= 2;
   const TopRoom room = top_room(k, size);
   const size_t other = (room.kept + room.ranked) * sizeof(TopKey), unit = (size_t)threads * 16 * (z.dtype == RT_DT_F32 ? 4 : 2);
-  const int places = (int)std::min(((threads == 256 ? 70 : 208) * 1024 - other) / unit, (size_t)VR_MAX_BLOCKS);
+  const int places = (int)std::min(((threads == 256 ? 70 : 208) * 1024 - other) / unit, (size_t)VR_MAX_UNITS);
   return with_dtype(z.dtype, [&](auto* zt) {
     return with_threads(threads, [&](auto n) {
       using T = std::remove_pointer_t<decltype(zt)>;

@@ -1,55 +1,228 @@
-// Softmax and distillation over rows of logits: a cluster of CTAs a row, each element read once.
+// Softmax and distillation over rows of logits.  A row is read once: it lies in the shared memory of a cluster of CTAs until its sums have
+// gone round.  In each CTA some warps sum row n + 1 while others write row n and the next ones are copied, so that memory is busy while sums
+// are found and go round, and a warp or a few make each row's list ready and find its loss.  (All warps at one row after the other, with
+// the same copies ahead, took 255 us for the gradients of 1024 x 151936 f32 logits.)
+//
+// What passes between the roles, row i of a CTA (all of them mbarriers, two or four in turn):
+//   full, empty   a unit has been copied; the warps that write the row (or, for a loss alone, that sum it) give it back
+//   patched       the list's warps have taken the listed elements out of the row
+//   summed        the row's exponentials and references are there
+//   exchange      all CTAs' sums of the row, and what their lists say, have come
+//   written       by the warps that write
+//   done          the row has been written, its listed elements too, and its loss found; row i + 2 may take its references' and its list's places.
+//                 Its sums are sent after that: whoever has seen exchange i - 2 complete knows that every CTA is done with row i - 4, whose
+//                 place the sums of row i take there
 #include "vocab_rows.cuh"
 
 namespace rt {
 
+constexpr int ROW_STEP = 2;  // vectors of a thread in a unit
+struct RowBars {
+  uint64_t units[2 * VR_MAX_UNITS], exchange[4], summed[2], written[2], done[2], patched[2];
+};
 // What a warp knows of its share of a row, and sends to every CTA of the cluster: a reference, and the sum of exponentials relative to it.
-struct alignas(8) SoftmaxStat {
+struct alignas(8) RowStat {
   float m, s;
 };
+__device__ __forceinline__ void row_wait_turn(uint64_t* bars, uint32_t i, uint32_t turns_log2, int* status) {
+  row_wait(bars + (i & ((1u << turns_log2) - 1)), i >> turns_log2 & 1, status);
+}
 
-template <class T, class O, int NT>
-__global__ void __launch_bounds__(NT + 32, ctas_of(NT))
-softmax_rows_kernel(const T* z, size_t ld, size_t rows, int vocab, ExpT ex, O* prob, size_t prob_ld, int places, int* status) {
-  constexpr int WARPS = NT / 32;
-  extern __shared__ uint4 slots[];
-  __shared__ uint64_t bars[2 * VR_MAX_BLOCKS + 2];
-  __shared__ SoftmaxStat stats[2][VR_MAX_CLUSTER * WARPS];
+// The warps that sum.  The thread's reference is the largest of its first vectors: an exponential may be as large as 2^30 before it changes,
+// so that it rarely does.  KEEP (32-bit rows): the exponentials take their elements' place, for the warps that write.
+template <class T, int NT, bool KEEP>
+__device__ __forceinline__ void sum_rows(UnitRing<T, NT, ROW_STEP>& ring, const T* z, size_t ld, size_t rows, size_t row_step, const ExpT& ex, RowBars& b,
+                                         float (*refs)[NT], RowStat (*stats)[VR_MAX_CLUSTER * (NT / 32)], uint32_t bytes, bool listed, bool give_back) {
+  using Ring = UnitRing<T, NT, ROW_STEP>;
+  constexpr int VEC = Ring::VEC, WARPS = NT / 32;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  Exchange exchange;
-  Ring<T, NT> ring(slots, bars, places, status, z, ld, rows, vocab, exchange);
-  if (tid >= NT) {
-    if (tid == NT) ring.copy_rows();
-    return;
-  }
-  const int warps = ring.size * WARPS;
-  for (size_t r = cluster_id(); r < rows; r += ring.row_step) {
-    const RowPart<T, NT> part = ring.part(r);
-    ring.wait_all(part);
-    work_sync<NT>();
-    float mine, m;
-    const float sum = ring.template exponentials<sizeof(T) == 4>(part, ex, &mine), warp_sum = warp_join(mine, sum, ex, &m);
-    fence_proxy_async_smem();  // what was written in the blocks comes before the copies that follow
-    SoftmaxStat* stat = stats[exchange.turn()];
-    if (tid == 0) exchange.expect(warps * sizeof(SoftmaxStat));
+  const float most = 30.0f / ex.hi;
+  uint32_t i = 0;
+  for (size_t r = cluster_id(); r < rows; r += row_step, ++i) {
+    ring.begin(z + r * ld);
+    if (i >= 2) row_wait_turn(b.done, i - 2, 1, ring.status);
+    if (listed) row_wait_turn(b.patched, i, 1, ring.status);
+    const int first_place = ring.place;
+    float ref = -INFINITY;
+    F2 acc[4] = {0, 0, 0, 0};
+#pragma unroll 1
+    for (int u = 0; u < ring.n_units; ++u) {
+      ring.wait();
+      uint4* const at = ring.unit() + tid;
+      if (!listed && (u == 0 || u + 1 == ring.n_units)) ring.complete(u, at);
+      const uint4 v[2] = {at[0], at[NT]};
+      float top;
+      if constexpr (sizeof(T) == 4) {
+        top = max_nan(__uint_as_float(v[0].x), __uint_as_float(v[0].y), max_nan(__uint_as_float(v[0].z), __uint_as_float(v[0].w)));
+        top = max_nan(max_nan(top, __uint_as_float(v[1].x), __uint_as_float(v[1].y)), __uint_as_float(v[1].z), __uint_as_float(v[1].w));
+      } else {
+        using T2 = std::conditional_t<std::is_same<T, __half>::value, __half2, __nv_bfloat162>;
+        T2 m = __hmax2_nan(__hmax2_nan(*(const T2*)&v[0].x, *(const T2*)&v[0].y), __hmax2_nan(*(const T2*)&v[0].z, *(const T2*)&v[0].w));
+        m = __hmax2_nan(m, __hmax2_nan(__hmax2_nan(*(const T2*)&v[1].x, *(const T2*)&v[1].y), __hmax2_nan(*(const T2*)&v[1].z, *(const T2*)&v[1].w)));
+        top = max_nan(to_f32(m.x), to_f32(m.y));
+      }
+      if (!(top <= ref + most) && ref == ref) {  // the first finite ones, ones that are far larger, a NaN, which stays
+        if (ref > -INFINITY) {
+          const float by = ex(ref - top);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[j] = mul2(acc[j], pack2(by, by));
+          if constexpr (KEEP) {
+#pragma unroll 1
+            for (int k = 0, place = first_place; k < u; ++k) {
+#pragma unroll
+              for (int j = 0; j < ROW_STEP; ++j) {
+                float4* e = (float4*)(ring.slots + place * Ring::UNIT + j * NT + tid);
+                *e = make_float4(e->x * by, e->y * by, e->z * by, e->w * by);
+              }
+              if (++place == ring.places) place = 0;
+            }
+          }
+        }
+        ref = top;
+      }
+      const float base = ref > -INFINITY ? -ref : 0.0f;
+      const F2 minus_ref = pack2(base, base);
+#pragma unroll
+      for (int j = 0; j < ROW_STEP; ++j) {
+        float x[VEC];
+        unpack_vector<T>(v[j], x);
+#pragma unroll
+        for (int k = 0; k < VEC; k += 2) {
+          ex.pair(pack2(x[k], x[k + 1]), minus_ref, x + k, x + k + 1);
+          acc[(j * VEC + k) / 2 & 3] = add2(acc[(j * VEC + k) / 2 & 3], pack2(x[k], x[k + 1]));
+        }
+        if constexpr (KEEP) at[j * NT] = make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
+      }
+      if (give_back) ring.release();
+      ring.next();
+    }
+    refs[i & 1][tid] = ref;
+    fence_proxy_async_smem();  // what was written in the units comes before the copies that follow
+    __syncwarp();
+    if (lane == 0) mbar_arrive(b.summed + (i & 1));
+    float x, y, m;
+    unpack2(add2(add2(acc[0], acc[1]), add2(acc[2], acc[3])), &x, &y);
+    const float s = warp_join(ref, x + y, ex, &m);
+    if (i >= 2) row_wait_turn(b.exchange, i - 2, 2, ring.status);
+    if (tid == 0) mbar_expect_tx(b.exchange + (i & 3), bytes);
     if (lane < ring.size)
-      send(mapa_u32(smem_u32(&stat[ring.rank * WARPS + warp]), lane), exchange.bar(lane), __float_as_uint(m), __float_as_uint(warp_sum));
-    exchange.wait();
-    const float row_sum = (float)warp_sum_f64(lane_join(warps, [&](int i, float* mi, float* si) { *mi = stat[i].m, *si = stat[i].s; }, ex, &m));
-    // a row of -inf has no probabilities, one with a NaN or +inf no number for them
-    ring.put_exponentials(part, prob + r * prob_ld, mine, m, m == -INFINITY ? 0.0f : m < INFINITY ? 1.0f / row_sum : NAN, ex);
-    ring.advance(part.n_it, true);
+      send(mapa_u32(smem_u32(&stats[i & 3][ring.rank * WARPS + warp]), lane), mapa_u32(smem_u32(b.exchange + (i & 3)), lane), __float_as_uint(m), __float_as_uint(s));
   }
 }
 
-// As above, of the elements outside of the teacher's list (m, s); the sum of those on it, relative to the largest logit listed; and the
-// teacher's mass on it.
-struct alignas(16) DistillStat {
-  double listed, mass;
-  float m, s;
+// One row's results into `out`, by the warps that write: (16-bit rows) e f, e the exponentials relative to the row's reference, or (32-bit rows, whose
+// exponentials are there relative to the thread's reference `mine`) those times what that makes f.  Gives the units back.
+template <class O, class T, int NT>
+__device__ __forceinline__ void write_row(UnitRing<T, NT, ROW_STEP>& ring, O* out, float mine, float reference, float f, const ExpT& ex) {
+  using Ring = UnitRing<T, NT, ROW_STEP>;
+  constexpr int VEC = Ring::VEC;
+  const bool aligned = ((uintptr_t)out - (uintptr_t)ring.align * sizeof(O)) % (VEC * sizeof(O) < 16 ? VEC * sizeof(O) : 16) == 0;
+  const float ref = reference > -INFINITY ? reference : 0.0f;
+  // in two factors: what is left of an exponential of 2^30 may be 2^30 larger than what one factor can say
+  const float h = sizeof(T) == 4 && mine > -INFINITY ? ex(0.5f * (mine - reference)) : 1.0f;
+  f *= h;
+  const F2 minus_ref = pack2(-ref, -ref), by = pack2(f, f), half_way = pack2(h, h);
+#pragma unroll 1
+  for (int u = 0; u < ring.n_units; ++u) {
+    ring.wait();
+    const uint4* const at = ring.unit() + threadIdx.x % NT;
+    const uint4 v[2] = {at[0], at[NT]};
+    ring.release();
+    ring.next();
+    const int c = ring.column(u, 0);
+#pragma unroll
+    for (int j = 0; j < ROW_STEP; ++j) {
+      float x[VEC];
+      unpack_vector<T>(v[j], x);
+#pragma unroll
+      for (int k = 0; k < VEC; k += 2) {
+        if constexpr (sizeof(T) != 4) ex.pair(pack2(x[k], x[k + 1]), minus_ref, x + k, x + k + 1);
+        F2 e = pack2(x[k], x[k + 1]);
+        if constexpr (sizeof(T) == 4) e = mul2(e, half_way);
+        unpack2(mul2(e, by), x + k, x + k + 1);
+      }
+      const int cj = c + j * NT * VEC;
+      if (aligned && ((u > 0 && u + 1 < ring.n_units) || (cj >= 0 && cj + VEC <= ring.vocab))) put_vector<O, VEC>(out + cj, x);
+      else put_elements<O, VEC>(out, cj, ring.vocab, x);
+    }
+  }
+}
+
+template <class T, class O, int NT>
+__global__ void __maxnreg__(NT == 256 ? 96 : 72)
+softmax_rows_kernel(const T* z, size_t ld, size_t rows, int vocab, ExpT ex, O* prob, size_t prob_ld, int places, int* status) {
+  constexpr int WARPS = NT / 32;
+  extern __shared__ uint4 slots[];
+  __shared__ RowBars b;
+  __shared__ RowStat stats[4][VR_MAX_CLUSTER * WARPS];
+  __shared__ float refs[2][NT];
+  const int tid = threadIdx.x;
+  UnitRing<T, NT, ROW_STEP> ring(slots, b.units, places, status, vocab);
+  if (tid < 4) mbar_init(b.exchange + tid, 1);
+  if (tid < 2) {
+    mbar_init(b.summed + tid, WARPS);
+    mbar_init(b.done + tid, WARPS);
+  }
+  mbar_fence_init();
+  cluster_sync_all();  // nobody sends to a CTA that does not run yet
+  const size_t row_step = gridDim.x / (unsigned)ring.size;
+  const int warps = ring.size * WARPS;
+  if (tid < NT) {
+    sum_rows<T, NT, sizeof(T) == 4>(ring, z, ld, rows, row_step, ex, b, refs, stats, warps * sizeof(RowStat), false, false);
+  } else if (tid < 2 * NT) {
+    uint32_t i = 0;
+    for (size_t r = cluster_id(); r < rows; r += row_step, ++i) {
+      ring.begin(z + r * ld);
+      row_wait_turn(b.exchange, i, 2, status);
+      const RowStat* stat = stats[i & 3];
+      float m;
+      const float sum = (float)warp_sum_f64(lane_join(warps, [&](int w, float* mi, float* si) { *mi = stat[w].m, *si = stat[w].s; }, ex, &m));
+      // a row of -inf has no probabilities, one with a NaN or +inf no number for them
+      const float f = m == -INFINITY ? 0.0f : m < INFINITY ? 1.0f / sum : NAN;
+      row_wait_turn(b.summed, i, 1, status);
+      write_row(ring, prob + r * prob_ld, refs[i & 1][tid - NT], m, f, ex);
+      __syncwarp();
+      if ((tid & 31) == 0) mbar_arrive(b.done + (i & 1));
+    }
+  } else if (tid == 2 * NT) {
+    ring.copy_rows(z, ld, rows, row_step);
+  }
+}
+
+// What a CTA's list says of a row: the sum of its listed elements' exponentials, relative to the largest logit listed; what the teacher has
+// left (-1: the list has no mass that the student could learn from); by what its probabilities are divided, inverted; the largest logit.
+struct alignas(16) ListStat {
+  double listed;
+  float rest, by;
+  float top, unused[3];
   static constexpr int SENT = 24;
 };
-static_assert(sizeof(DistillStat) == 32, "sent as 16 and 8 bytes, which have to be aligned");
+struct alignas(16) LossStat {  // the teacher's mass, and sum q (t_j - z_j / T), the z relative to the largest
+  double mass, cross;
+};
+// What a row's sums make of it: a gradient outside of the list is exp(z - reference) outside, one on it e listed - q by, e relative to the largest listed.
+struct RowGradient {
+  float reference, outside, listed, by;
+  bool idle;
+};
+template <int WARPS>
+__device__ __forceinline__ RowGradient row_gradient(const RowStat* stat, const ListStat* list, int size, float w, float t, bool scaled, const ExpT& ex) {
+  RowGradient g;
+  float mo, on = 0.0f;
+  float so = (float)lane_join(size * WARPS, [&](int i, float* mi, float* si) { *mi = stat[i].m, *si = stat[i].s; }, ex, &mo);
+  so = warp_sum_f32(so);
+  for (int i = 0; i < size; ++i) on += (float)list[i].listed;
+  const float top = list[0].top, rest = list[0].rest, m = max_nan(mo, top), by = scaled ? 1.0f : w / t;
+  const bool bad = !(m < INFINITY);
+  const float rest_to = mo > -INFINITY ? ex(mo - m) : 0.0f, top_to = top > -INFINITY ? ex(top - m) : 0.0f;
+  const float inv = 1.0f / (so * rest_to + on * top_to);
+  g.reference = mo;
+  g.outside = bad ? NAN : so > 0.0f ? (rest_to * inv - rest / so) * by : 0.0f;
+  g.listed = bad ? NAN : m > -INFINITY ? top_to * inv * by : 0.0f;
+  g.by = list[0].by * by;
+  g.idle = w == 0.0f || rest < 0.0f;
+  return g;
+}
 
 // An element on the list leaves the row, whose sums and results are then those outside of the list: -inf in its place.  Returns whether
 // another entry may have taken it before.
@@ -67,210 +240,283 @@ __device__ __forceinline__ bool take_out(uint4* slots, int element) {
   }
 }
 
-
-// What 64 bits cost here is latency, of exp, log and division some 1000 cycles each: the two exponentials of an entry stand side by side,
-// logarithms and divisions wait for the loss, which a warp finds while the others go on with the next row.
+// One entry a thread of the list's warps.  64 bits for what is left of the teacher's mass, a difference, and for the loss, a small difference of
+// large sums; for those alone, since exp, log and division take some 1000 cycles each there.
 template <class T, class O, int NT>
-__global__ void __launch_bounds__(NT + 32, ctas_of(NT))
+__global__ void __maxnreg__(72)
 distill_rows_kernel(const T* z, size_t ld, size_t rows, int vocab, float t, ExpT ex, const int* index, const float* teacher, int k, int tail,
                     const float* weight, float* loss, O* d, size_t d_ld, float* row_scale, int places, int* status) {
-  constexpr int WARPS = NT / 32, LIST_WARPS = RT_TOP_MAX / 32;
+  using Ring = UnitRing<T, NT, ROW_STEP>;
+  constexpr int WARPS = NT / 32, LIST_WARPS = RT_TOP_MAX / 32, VEC = Ring::VEC;
   extern __shared__ uint4 slots[];
-  __shared__ uint64_t bars[2 * VR_MAX_BLOCKS + 2];
-  __shared__ DistillStat stats[2][VR_MAX_CLUSTER * WARPS];
-  __shared__ double s_cross[2][LIST_WARPS], s_q[RT_TOP_MAX];
+  __shared__ RowBars b;
+  __shared__ RowStat stats[4][VR_MAX_CLUSTER * WARPS];
+  __shared__ ListStat lists[4][VR_MAX_CLUSTER];
+  __shared__ LossStat losses[4];
+  __shared__ float refs[2][NT];
+  __shared__ double s_e[2][RT_TOP_MAX], s_q[2][RT_TOP_MAX], s_sums[LIST_WARPS][3];
+  __shared__ int s_mine[2][RT_TOP_MAX];  // the entry's column, if it is in this CTA's units and no entry before it has it, or -1
   __shared__ float s_top[LIST_WARPS];
   __shared__ int s_index[RT_TOP_MAX];
-  static_assert(RT_TOP_MAX <= NT);
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, list_warps = (k + 31) / 32;
-  Exchange exchange;
-  Ring<T, NT> ring(slots, bars, places, status, z, ld, rows, vocab, exchange);
-  if (tid >= NT) {
-    if (tid == NT) ring.copy_rows();
-    return;
+  const int tid = threadIdx.x, lane = tid & 31, list_warps = (k + 31) / 32;
+  Ring ring(slots, b.units, places, status, vocab);
+  const bool finds_loss = loss && ring.rank == 0;
+  if (tid < 4) mbar_init(b.exchange + tid, 1);
+  if (tid < 2) {
+    mbar_init(b.summed + tid, WARPS);
+    mbar_init(b.written + tid, WARPS);
+    mbar_init(b.done + tid, 1);
+    mbar_init(b.patched + tid, list_warps);
   }
-  const double inv_t = 1.0 / t;
-  const bool with_entries = warp < list_warps;
-  const int warps = ring.size * WARPS;
-  // The thread's entry of the list: its index (-1: none), the teacher's log-probability, the student's logit.
-  auto entry = [&](size_t r, float* tl) {
-    *tl = tid < k ? teacher[r * k + tid] : 0.0f;
-    return tid < k ? index[r * k + tid] : -1;
-  };
-  auto logit = [&](size_t r, int* i) {
-    if (*i < -1 || *i >= vocab) {
-      if (ring.rank == 0) report_status(status, RT_ERR_BAD_INDEX);
-      *i = -1;
-    }
-    return *i >= 0 ? to_f32(z[r * ld + *i]) : -INFINITY;
-  };
-  size_t r = cluster_id();
-  float w = weight ? weight[r] : 1.0f, tl;
-  int my = entry(r, &tl);
-  float z_my = logit(r, &my);
-  for (size_t next_r; r < rows; r = next_r) {
-    next_r = r + ring.row_step;
-    const bool more = next_r < rows;
-    const RowPart<T, NT> part = ring.part(r);
-    const float factor = w / t, g = row_scale ? 1.0f : factor;
-    O* out = d ? d + r * d_ld : nullptr;
-    if (row_scale && tid == 0 && ring.rank == 0) row_scale[r] = factor;
-    float next_tl = 0.0f, next_w = 1.0f, next_z = -INFINITY;
-    int next_my = -1;
-    if (more) {
-      next_my = entry(next_r, &next_tl);
-      if (weight) next_w = weight[next_r];
-    }
-    auto no_gradient = [&] {
-      if (out)
-        ring.put(part, out, [](const uint4&, float* x) {
-#pragma unroll
-          for (int i = 0; i < RowPart<T, NT>::VEC; ++i) x[i] = 0.0f;
-        });
-      else
-        ring.release_all(part);
-      if (loss && tid == 0 && ring.rank == 0) loss[r] = 0.0f;
-    };
-    // the list leaves the row
-    int it_my = 0, element = 0;
-    bool first = my >= 0 && part.owner(my, &it_my, &element) == ring.rank, again = false;
-    if (with_entries) {
-      const float warp_top = warp_max_nan(z_my);
-      if (lane == 0) s_top[warp] = warp_top;
-      if (tid < k) s_index[tid] = my;
-    }
-    ring.wait_all(part);
-    work_sync<NT>();
-    float top = -INFINITY;  // the largest logit listed
-    for (int i = 0; i < list_warps; ++i) top = max_nan(top, s_top[i]);
-    if (first) again = take_out<T>(ring.block(it_my), element);
-    again = work_sync_or<NT>(again);
-    if (w == 0.0f) {  // nothing to learn from, whatever the logits are
-      fence_proxy_async_smem();
-      work_sync<NT>();
-      no_gradient();
-      if (more) next_z = logit(next_r, &next_my);
-    } else {
-      DistillStat st{0.0, 0.0, -INFINITY, 0.0f};
-      double q = 0.0, e_my = 0.0;  // 64 bits for what is left of the mass, a difference, and for the loss
-      double q_all = 0.0;
-      if (with_entries) {
-        const double x_my = z_my > -INFINITY ? (z_my == top ? 0.0 : ((double)z_my - top) * inv_t) : -INFINITY, lt = tl;
-        if (my >= 0) q = exp(lt), e_my = exp(x_my);
-        q_all = q;
-        if (again && tid < k) s_q[tid] = q;
-        double cross = q > 0.0 ? q * (lt - x_my) : 0.0;  // sum q (t_j - z_j / T), the z relative to the largest
-        st.mass = q;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) st.mass += __shfl_xor_sync(0xffffffffu, st.mass, o), cross += __shfl_xor_sync(0xffffffffu, cross, o);
-        if (lane == 0) s_cross[exchange.turn()][warp] = cross;
-      }
-      if (again) {  // an index came twice: its first entry answers for all of them
-        work_sync<NT>();
-        if (first) {
-          q_all = 0.0;
-          for (int j = 0; j < k; ++j)
-            if (s_index[j] == my) {
-              if (j < tid) first = false;
-              q_all += s_q[j];
-            }
+  mbar_fence_init();
+  cluster_sync_all();  // nobody sends to a CTA that does not run yet
+  const size_t row_step = gridDim.x / (unsigned)ring.size;
+  const int warps = ring.size * WARPS, writers = d ? NT : 0, copier = NT + writers, finisher = copier + 32, lister = finisher + 32;
+  if (tid < NT) {
+    const uint32_t bytes = warps * sizeof(RowStat) + ring.size * ListStat::SENT + (finds_loss ? sizeof(LossStat) : 0);
+    if (d) sum_rows<T, NT, sizeof(T) == 4>(ring, z, ld, rows, row_step, ex, b, refs, stats, bytes, true, false);
+    else sum_rows<T, NT, false>(ring, z, ld, rows, row_step, ex, b, refs, stats, bytes, true, true);
+  } else if (tid < copier) {  // writes
+    uint32_t i = 0;
+    for (size_t r = cluster_id(); r < rows; r += row_step, ++i) {
+      const float w = weight ? weight[r] : 1.0f;
+      ring.begin(z + r * ld);
+      row_wait_turn(b.exchange, i, 2, status);
+      const RowGradient g = row_gradient<WARPS>(stats[i & 3], lists[i & 3], ring.size, w, t, row_scale != nullptr, ex);
+      row_wait_turn(b.summed, i, 1, status);
+      // (rows that nothing is learnt from, whatever their logits are, have zeros)
+      if (!g.idle) {
+        write_row(ring, d + r * d_ld, refs[i & 1][tid - NT], g.reference, g.outside, ex);
+      } else {
+        for (int u = 0; u < ring.n_units; ++u, ring.next()) {
+          const float zero[VEC] = {};
+          for (int j = 0; j < ROW_STEP; ++j) put_elements<O, VEC>(d + r * d_ld, ring.column(u, j), vocab, zero);
+          ring.release();
         }
       }
-      if (with_entries) st.listed = warp_sum_f64(first ? e_my : 0.0);
-      float mine;
-      const float sum = out ? ring.template exponentials<sizeof(T) == 4>(part, ex, &mine) : ring.template exponentials<false>(part, ex, &mine);
-      st.s = warp_join(mine, sum, ex, &st.m);
-      fence_proxy_async_smem();  // what was written in the blocks comes before the copies that follow
-      DistillStat* stat = stats[exchange.turn()];
-      const double* all_cross = s_cross[exchange.turn()];
-      if (tid == 0) exchange.expect(warps * DistillStat::SENT);
-      if (lane < ring.size) {
-        const uint32_t to = mapa_u32(smem_u32(&stat[ring.rank * WARPS + warp]), lane), bar = exchange.bar(lane);
-        const uint2 a = *(const uint2*)&st.listed, b = *(const uint2*)&st.mass;
-        send(to, bar, a.x, a.y, b.x, b.y);
-        send(to + 16, bar, __float_as_uint(st.m), __float_as_uint(st.s));
-      }
-      exchange.wait();
-      if (more) next_z = logit(next_r, &next_my);
-      double mass = 0.0;  // every CTA has found the same
-      for (int i = 0; i < list_warps; ++i) mass += stat[i].mass;
-      const bool idle = !tail && mass == 0.0;
-      const double rest = tail ? fmax(0.0, 1.0 - mass) : 0.0;
-      // the sums of what is outside, relative to mo, and of what is listed, relative to top: in 32 bits for the gradients
-      float mo, listed = 0.0f;
-      const double lane_so = lane_join(warps, [&](int i, float* mi, float* si) { *mi = stat[i].m, *si = stat[i].s, listed += (float)stat[i].listed; }, ex, &mo);
-      const float m = max_nan(mo, top);
-      const bool bad = !(m < INFINITY);
-      if (idle) {
-        no_gradient();
-      } else if (out) {
-        float so = (float)lane_so;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) so += __shfl_xor_sync(0xffffffffu, so, o), listed += __shfl_xor_sync(0xffffffffu, listed, o);
-        // a gradient outside of the list is exp(z - mo) co, one on it e to - q by, e relative to the largest listed
-        const float rest_to = mo > -INFINITY ? ex(mo - m) : 0.0f, top_to = top > -INFINITY ? ex(top - m) : 0.0f;
-        const float inv = 1.0f / (so * rest_to + listed * top_to);
-        const float co = bad ? NAN : so > 0.0f ? (rest_to * inv - (float)rest / so) * g : 0.0f;
-        const float to = bad ? NAN : m > -INFINITY ? top_to * inv * g : 0.0f, by = tail ? g : g / (float)mass;
-        ring.put_exponentials(part, out, mine, mo, co, ex);
-        work_sync<NT>();  // what is on the list overwrites what its vector's thread wrote
-        if (first) out[my] = from_f32<O>((float)(e_my * to - q_all * by));
-      }
-      if (!out && !idle) ring.release_all(part);
-      if (loss && !idle && ring.rank == 0 && warp == WARPS - 1) {
-        double so = lane_so, listed64 = 0.0, cross = lane < list_warps ? all_cross[lane] : 0.0;
-        for (int i = lane; i < warps; i += 32) listed64 += stat[i].listed;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-          so += __shfl_xor_sync(0xffffffffu, so, o);
-          listed64 += __shfl_xor_sync(0xffffffffu, listed64, o);
-          cross += __shfl_xor_sync(0xffffffffu, cross, o);
-        }
-        // log(listed + outside), the first relative to `top`, the second to mo, log(outside), log(rest) and log(mass): side by side
+      __syncwarp();
+      if (lane == 0) mbar_arrive(b.written + (i & 1));
+    }
+  } else if (tid < finisher) {
+    if (tid == copier) ring.copy_rows(z, ld, rows, row_step);
+  } else if (tid < lister) {  // finds the loss, and writes the gradients on the list over what was written there
+    const double inv_t = 1.0 / t;
+    uint32_t i = 0;
+    for (size_t r = cluster_id(); r < rows; r += row_step, ++i) {
+      const float w = weight ? weight[r] : 1.0f;
+      row_wait_turn(b.exchange, i, 2, status);
+      const RowStat* stat = stats[i & 3];
+      const ListStat* list = lists[i & 3];
+      if (finds_loss) {
+        const double mass = losses[i & 3].mass, cross = losses[i & 3].cross;
+        const float top = list[0].top;
+        float mo;
+        double so = lane_join(warps, [&](int w, float* mi, float* si) { *mi = stat[w].m, *si = stat[w].s; }, ex, &mo), on = 0.0;
+        so = warp_sum_f64(so);
+        for (int c = 0; c < ring.size; ++c) on += list[c].listed;
+        const double rest = tail ? fmax(0.0, 1.0 - mass) : 0.0;
+        // log(on + outside), the first relative to `top`, the second to mo, log(outside), log(rest) and log(mass): side by side
         const double x = ((double)mo - top) * inv_t;  // of the outside, in units of `top`
         const bool above = !(x <= 0.0) && mo > -INFINITY;
         const double shrink = above ? (top > -INFINITY ? exp(-x) : 0.0) : (mo > -INFINITY ? exp(x) : 0.0);
-        const double log_of = log(lane == 0 ? (above ? so + listed64 * shrink : listed64 + so * shrink) : lane == 1 ? so : lane == 2 ? rest : mass);
+        const double log_of = log(lane == 0 ? (above ? so + on * shrink : on + so * shrink) : lane == 1 ? so : lane == 2 ? rest : mass);
         const double log_sum = __shfl_sync(0xffffffffu, log_of, 0), log_so = __shfl_sync(0xffffffffu, log_of, 1), log_rest = __shfl_sync(0xffffffffu, log_of, 2),
                      log_mass = __shfl_sync(0xffffffffu, log_of, 3);
         if (lane == 0) {
           double l = mass == 0.0 ? 0.0 : top > -INFINITY ? cross + mass * (log_sum + (above ? x : 0.0)) : INFINITY;
           if (!tail) l = l / mass - log_mass;
           if (rest > 0.0) l += so > 0.0 ? rest * (log_rest - log_so + log_sum - (above ? 0.0 : x)) : INFINITY;
-          loss[r] = bad ? NAN : (float)(w * l);
+          loss[r] = w == 0.0f || (!tail && mass == 0.0) ? 0.0f : !(max_nan(mo, top) < INFINITY) ? NAN : (float)(w * l);
         }
       }
+      if (d) {
+        const RowGradient g = row_gradient<WARPS>(stat, list, ring.size, w, t, row_scale != nullptr, ex);
+        row_wait_turn(b.written, i, 1, status);
+        for (int j = lane; j < k; j += 32) {
+          const int c = s_mine[i & 1][j];
+          if (c >= 0 && !g.idle) d[r * d_ld + c] = from_f32<O>((float)(s_e[i & 1][j] * g.listed - s_q[i & 1][j] * g.by));
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(b.done + (i & 1));
     }
-    ring.advance(part.n_it, true);
-    w = next_w;
-    my = next_my;
-    tl = next_tl;
-    z_my = next_z;
+  } else {  // makes the lists ready, a row ahead or two
+    const int me = tid - lister, warp = me >> 5, threads = list_warps * 32;
+    const double inv_t = 1.0 / t;
+    auto list_sync = [&] { asm volatile("bar.sync 2, %0;" ::"r"(threads) : "memory"); };
+    auto list_sync_or = [&](bool v) {
+      uint32_t any;
+      asm volatile(
+          "{\n\t.reg .pred p, q;\n\t"
+          "setp.ne.u32 p, %1, 0;\n\t"
+          "bar.red.or.pred q, 2, %2, p;\n\t"
+          "selp.u32 %0, 1, 0, q;\n\t}"
+          : "=r"(any)
+          : "r"((uint32_t)v), "r"(threads)
+          : "memory");
+      return any != 0;
+    };
+    // The thread's entry: its index (-1: none), the teacher's log-probability, the student's logit.
+    auto entry = [&](size_t r, float* tl) {
+      *tl = me < k ? teacher[r * k + me] : 0.0f;
+      return me < k ? index[r * k + me] : -1;
+    };
+    auto logit = [&](size_t r, int* i) {
+      if (*i < -1 || *i >= vocab) {
+        if (ring.rank == 0) report_status(status, RT_ERR_BAD_INDEX);
+        *i = -1;
+      }
+      return *i >= 0 ? to_f32(z[r * ld + *i]) : -INFINITY;
+    };
+    size_t r = cluster_id();
+    float tl;
+    int my = entry(r, &tl);
+    float z_my = logit(r, &my);
+    for (uint32_t i = 0; r < rows; ++i) {
+      const size_t next_r = r + row_step;
+      float next_tl = 0.0f;
+      const int next_entry = next_r < rows ? entry(next_r, &next_tl) : -1;
+      if (i >= 2) row_wait_turn(b.exchange, i - 2, 2, status);  // not further ahead: the barriers tell two rows apart
+      ring.begin(z + r * ld);
+      if (row_scale && me == 0 && ring.rank == 0) row_scale[r] = (weight ? weight[r] : 1.0f) / t;
+      auto place_of = [&](int u, uint32_t* phase) {
+        const int n = ring.place + u;
+        *phase = ring.phase ^ (n < ring.places ? 0u : 1u);
+        return n < ring.places ? n : n - ring.places;
+      };
+      uint32_t phase;
+      const float warp_top = warp_max_nan(z_my);
+      if (lane == 0) s_top[warp] = warp_top;
+      s_index[me] = my;
+      for (int u = warp; u < ring.n_units; u += list_warps) {
+        const int p = place_of(u, &phase);
+        row_wait(ring.full + p, phase, status);
+      }
+      list_sync();
+      float top = -INFINITY;  // the largest logit listed
+      for (int j = 0; j < list_warps; ++j) top = max_nan(top, s_top[j]);
+      // vectors that stick out of the row, and what is behind its last one
+      if (ring.n_units > 0) {
+        if (me == 0 && ring.rank == 0 && ring.align) ring.complete_vector(0, 0, ring.slots + place_of(0, &phase) * Ring::UNIT);
+        const int u = ring.n_units - 1, at = ring.first_vector(u), end_whole = (ring.align + vocab) / VEC;
+        uint4* const unit = ring.slots + place_of(u, &phase) * Ring::UNIT;
+        for (int v = max(end_whole - at, 0) + me; v < Ring::UNIT; v += threads) ring.complete_vector(u, v, unit + v);
+      }
+      list_sync();
+      bool first = false, again = false;
+      if (my >= 0) {
+        const int v = (my + ring.align) / VEC;
+        const unsigned unit = v / Ring::UNIT, u = unit / (unsigned)ring.size;
+        first = (int)(unit - u * ring.size) == ring.rank;
+        if (first) again = take_out<T>(ring.slots + place_of((int)u, &phase) * Ring::UNIT, (v % Ring::UNIT) * VEC + (my + ring.align) % VEC);
+      }
+      again = list_sync_or(again);
+      fence_proxy_async_smem();  // what was written in the units comes before the copies that follow
+      __syncwarp();
+      if (lane == 0) mbar_arrive(b.patched + (i & 1));
+      int next_my = next_entry;
+      const float next_z = next_r < rows ? logit(next_r, &next_my) : -INFINITY;
+      // the list's sums
+      const double x_my = z_my > -INFINITY ? (z_my == top ? 0.0 : ((double)z_my - top) * inv_t) : -INFINITY, lt = tl;
+      double q = 0.0, e = 0.0;
+      if (my >= 0) q = exp(lt), e = exp(x_my);
+      if (i >= 2) row_wait_turn(b.done, i - 2, 1, status);
+      s_e[i & 1][me] = e;
+      s_q[i & 1][me] = q;
+      if (again) {  // an index came twice: its first entry answers for all of them
+        list_sync();
+        double q_all = q;
+        if (first) {
+          q_all = 0.0;
+          for (int j = 0; j < k; ++j)
+            if (s_index[j] == my) {
+              if (j < me) first = false;
+              q_all += s_q[i & 1][j];
+            }
+        }
+        list_sync();
+        s_q[i & 1][me] = q_all;
+      }
+      s_mine[i & 1][me] = first ? my : -1;
+      double mass = q, cross = q > 0.0 ? q * (lt - x_my) : q, on = first ? e : 0.0;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        mass += __shfl_xor_sync(0xffffffffu, mass, o);
+        cross += __shfl_xor_sync(0xffffffffu, cross, o);
+        on += __shfl_xor_sync(0xffffffffu, on, o);
+      }
+      if (lane == 0) s_sums[warp][0] = mass, s_sums[warp][1] = cross, s_sums[warp][2] = on;
+      list_sync();
+      if (warp == 0) {
+        mass = cross = on = 0.0;
+        for (int j = 0; j < list_warps; ++j) mass += s_sums[j][0], cross += s_sums[j][1], on += s_sums[j][2];
+        const float rest = tail ? (float)fmax(0.0, 1.0 - mass) : mass == 0.0 ? -1.0f : 0.0f, by = tail ? 1.0f : 1.0f / (float)mass;
+        const uint64_t* bar = b.exchange + (i & 3);
+        if (lane < ring.size) {
+          const uint32_t to = mapa_u32(smem_u32(&lists[i & 3][ring.rank]), lane), its_bar = mapa_u32(smem_u32(bar), lane);
+          send(to, its_bar, (uint32_t)__double2loint(on), (uint32_t)__double2hiint(on), __float_as_uint(rest), __float_as_uint(by));
+          send(to + 16, its_bar, __float_as_uint(top), 0u);
+        }
+        if (finds_loss && lane == 0)
+          send(mapa_u32(smem_u32(&losses[i & 3]), 0), mapa_u32(smem_u32(bar), 0), (uint32_t)__double2loint(mass), (uint32_t)__double2hiint(mass),
+               (uint32_t)__double2loint(cross), (uint32_t)__double2hiint(cross));
+      }
+      ring.place += ring.n_units;
+      if (ring.place >= ring.places) ring.place -= ring.places, ring.phase ^= 1;
+      r = next_r, my = next_my, tl = next_tl, z_my = next_z;
+    }
   }
 }
 
+// How rows are held.  Threads that sum, and that write: 128 where that is no more than eight units of a row, else 256.  The CTAs of a row's cluster: as
+// few as hold two rows, one that is summed and one that is written (longer rows have eight and are held once, at least), more where there are so few
+// rows that SMs would be idle.  The ring's units: all that fit, as far as there are rows to fill them.
+struct RowShape {
+  int threads, cluster, places;
+  size_t smem;
+};
+static RowShape row_shape(const rt_ctx* c, size_t rows, int vocab, int dtype) {
+  const int vec = dtype == RT_DT_F32 ? 4 : 8, vectors = (vec - 1 + vocab + vec - 1) / vec;  // at the worst alignment
+  const int threads = vectors <= 2048 ? 128 : 256, units = (vectors + ROW_STEP * threads - 1) / (ROW_STEP * threads);
+  const size_t unit = (size_t)ROW_STEP * threads * 16, third = 66 * 1024, half = 100 * 1024, all = VR_MOST_SMEM;
+  int size = 1;
+  while (size * 2 <= VR_MAX_CLUSTER && units > size && rows * size * 2 <= (size_t)c->num_sms) size *= 2;
+  auto each = [&] { return (size_t)((units + size - 1) / size); };
+  while (size < VR_MAX_CLUSTER && 2 * each() * unit > all) ++size;
+  const size_t turns = (rows * size + c->num_sms - 1) / c->num_sms, want = each() * std::min(turns, (size_t)4);
+  const size_t room = 2 * each() * unit <= third ? third : 2 * each() * unit <= half ? half : all;
+  const size_t places = std::max(each(), std::min(std::min(room / unit, (size_t)VR_MAX_UNITS), want));
+  return {threads, size, (int)places, places * unit};
+}
+template <class F>
+static int with_row_threads(int threads, F&& f) {
+  if (threads == 128) return f(std::integral_constant<int, 128>());
+  return f(std::integral_constant<int, 256>());
+}
+
 int launch_softmax_rows(rt_ctx* c, const VocabRows& z, size_t rows, int vocab, float temperature, void* prob, int prob_dtype, size_t prob_ld) {
-  const RowShape shape = row_shape(c, rows, vocab, z.dtype, 0);
+  const RowShape shape = row_shape(c, rows, vocab, z.dtype);
   return with_dtype(z.dtype, [&](auto* zt) {
     return with_dtype(prob_dtype, [&](auto* ot) {
-      return with_threads(shape.threads, [&](auto threads) {
+      return with_row_threads(shape.threads, [&](auto threads) {
         using T = std::remove_pointer_t<decltype(zt)>;
         using O = std::remove_pointer_t<decltype(ot)>;
-        return launch_clusters(c, softmax_rows_kernel<T, O, decltype(threads)::value>, true, rows, shape.threads + 32, shape.cluster, shape.smem, (const T*)z.p, z.ld,
-                               rows, vocab, exp_t(temperature), (O*)prob, prob_ld, shape.places, c->status_dev);
+        return launch_clusters(c, softmax_rows_kernel<T, O, decltype(threads)::value>, true, rows, 2 * shape.threads + 32, shape.cluster, shape.smem,
+                               (const T*)z.p, z.ld, rows, vocab, exp_t(temperature), (O*)prob, prob_ld, shape.places, c->status_dev);
       });
     });
   });
 }
 
 int launch_distill_rows(rt_ctx* c, const DistillArgs& a, size_t rows) {
-  const RowShape shape = row_shape(c, rows, a.vocab, a.z.dtype, 0);
+  const RowShape shape = row_shape(c, rows, a.vocab, a.z.dtype);
+  const int all_threads = (a.d ? 2 : 1) * shape.threads + 64 + (a.k + 31) / 32 * 32;
   return with_dtype(a.z.dtype, [&](auto* zt) {
     return with_dtype(a.d_dtype, [&](auto* ot) {
-      return with_threads(shape.threads, [&](auto threads) {
+      return with_row_threads(shape.threads, [&](auto threads) {
         using T = std::remove_pointer_t<decltype(zt)>;
         using O = std::remove_pointer_t<decltype(ot)>;
-        return launch_clusters(c, distill_rows_kernel<T, O, decltype(threads)::value>, true, rows, shape.threads + 32, shape.cluster, shape.smem, (const T*)a.z.p,
+        return launch_clusters(c, distill_rows_kernel<T, O, decltype(threads)::value>, true, rows, all_threads, shape.cluster, shape.smem, (const T*)a.z.p,
                                a.z.ld, rows, a.vocab, a.temperature, exp_t(a.temperature), a.index, a.teacher, a.k, a.mode == RT_DISTILL_TAIL, a.weight,
                                a.loss, (O*)a.d, a.d_ld, a.row_scale, shape.places, c->status_dev);
       });

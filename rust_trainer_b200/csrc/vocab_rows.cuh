@@ -120,14 +120,12 @@ __device__ __forceinline__ void unpack_vector(const uint4& u, float* x) {
 
 // ---- rows on clusters
 // A row is cut into vectors of 16 aligned bytes (the first and the last may stick out of it: what is outside reads as -inf), these into
-// blocks of a vector a thread, and the blocks are dealt to the cluster's CTAs in turn, so that each sees a sample of the whole row
-// wherever its large values lie.  A warp beside the NT threads that work brings the blocks as bulk copies into a ring in shared memory, all
-// that find room there in flight at once; every element is read from memory once.  Clusters stay for as many rows as there are, and a
-// block's place takes one of the next row as soon as the last warp is done with it.  What a row costs beside its bytes (barriers, sums
-// that go round the cluster, lists: some microseconds a CTA) is paid by each of its CTAs, so that clusters are as small as can be:
-// three CTAs hold 151936 f32 logits.
-constexpr uint32_t VR_MOST_SMEM = 212 * 1024;  // dynamic shared memory of a CTA: what the kernels' fixed arrays, 13 KB at most, leave of 227
-constexpr int VR_MAX_CLUSTER = 8, VR_MAX_BLOCKS = 64;  // blocks of a ring
+// units of a few vectors a thread, and the units are dealt to the cluster's CTAs in turn, so that each sees a sample of the whole row
+// wherever its large values lie.  A warp that does nothing else brings the units as bulk copies into a ring in shared memory, all that
+// find room there in flight at once; every element is read from memory once.  Clusters stay for as many rows as there are, and a
+// unit's place takes one of the next row as soon as the last warp is done with it.
+constexpr uint32_t VR_MOST_SMEM = 208 * 1024;  // dynamic shared memory of a CTA: what the kernels' fixed arrays, 19 KB at most, leave of 227
+constexpr int VR_MAX_CLUSTER = 8, VR_MAX_UNITS = 64;  // units of a ring
 constexpr int SITE_VOCAB_ROW = 701;
 
 __device__ __forceinline__ size_t cluster_id() {
@@ -151,22 +149,10 @@ __device__ __forceinline__ void send(uint32_t to, uint32_t bar, uint32_t a, uint
 __device__ __forceinline__ void send(uint32_t to, uint32_t bar, double v) {
   asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.b64 [%0], %1, [%2];" ::"r"(to), "l"(__double_as_longlong(v)), "r"(bar) : "memory");
 }
-// barriers of the NT threads that work
+// barriers of some of a CTA's warps
 template <int NT>
 __device__ __forceinline__ void work_sync() { asm volatile("bar.sync 1, %0;" ::"n"(NT) : "memory"); }
-template <int NT>
-__device__ __forceinline__ bool work_sync_or(bool v) {
-  uint32_t r;
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\t"
-      "setp.ne.u32 p, %1, 0;\n\t"
-      "bar.red.or.pred q, 1, %2, p;\n\t"
-      "selp.u32 %0, 1, 0, q;\n\t}"
-      : "=r"(r)
-      : "r"((uint32_t)v), "n"(NT)
-      : "memory");
-  return r != 0;
-}
+
 // Waits for a phase of a barrier, asleep for up to some microseconds at a time: a warp that polls takes instructions from those that work.
 // The matmul's wait gives up when another kernel has reported anything; here an index out of range in one row must not end the
 // others' waits, so that only the time limit does.
@@ -193,36 +179,6 @@ static __device__ __noinline__ void row_wait_slow(uint64_t* bar, uint32_t phase,
 __device__ __forceinline__ void row_wait(uint64_t* bar, uint32_t phase, int* status) {
   if (!mbar_sleep(bar, phase)) row_wait_slow(bar, phase, status);
 }
-
-// Where a row's elements are: its vectors, and the blocks of them that are this CTA's.
-template <class T, int NT>
-struct RowPart {
-  static constexpr int VEC = 16 / (int)sizeof(T);   // elements of a vector
-  static constexpr int STEP = 16 / VEC;             // blocks that give a thread 16 elements
-  static constexpr uint32_t NONE = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;  // -inf
-  const T* row;
-  int vocab, rank, size, phase, n_vec, n_it;  // n_it: this CTA's blocks
-
-  __device__ __forceinline__ RowPart(const T* row_, int vocab_, int rank_, int size_) : row(row_), vocab(vocab_), rank(rank_), size(size_) {
-    phase = (int)(((uintptr_t)row & 15) / sizeof(T));
-    n_vec = (phase + vocab + VEC - 1) / VEC;
-    n_it = (int)((unsigned)((n_vec + NT - 1) / NT - rank + size - 1) / (unsigned)size);
-  }
-  __device__ __forceinline__ int first_vector(int it) const { return (it * size + rank) * NT; }
-  // the column of the first element of the thread's vector
-  __device__ __forceinline__ int column(int it) const { return (first_vector(it) + (int)threadIdx.x) * VEC - phase; }
-  // where column `c` lies: its CTA, its block there, and its place among the block's elements
-  __device__ __forceinline__ int owner(int c, int* it, int* element) const {
-    const int v = (c + phase) / VEC;
-    const unsigned block = v / NT;
-    *it = (int)(block / (unsigned)size);
-    *element = (v % NT) * VEC + (c + phase) % VEC;
-    return (int)(block - (unsigned)*it * size);
-  }
-  // whether the thread's vector of a block may not be whole: only the row's first and last vectors stick out
-  __device__ __forceinline__ bool outer(int it) const { return it == 0 || it + 1 == n_it; }
-  static __device__ __forceinline__ void unpack(const uint4& u, float* x) { unpack_vector<T>(u, x); }
-};
 
 // A vector's results: as a whole, where they lie on 16 bytes (8 where they are no longer), or what there is of them in a row of `vocab`.
 template <class O, int VEC>
@@ -263,6 +219,12 @@ struct Exchange {
   uint64_t* bars;  // [2]
   int* status;
   uint32_t n = 0;
+  __device__ __forceinline__ void begin(uint64_t* bars_, int* status_) {
+    bars = bars_;
+    status = status_;
+    if (threadIdx.x < 2) mbar_init(bars + threadIdx.x, 1);
+    mbar_fence_init();
+  }
   __device__ __forceinline__ int turn() const { return n & 1; }
   __device__ __forceinline__ uint32_t bar(uint32_t rank) const { return mapa_u32(smem_u32(bars + turn()), rank); }
   // what is to come, by one thread of the CTA (before or after it comes)
@@ -273,233 +235,85 @@ struct Exchange {
   }
 };
 
-// A CTA's ring of blocks.  Blocks are numbered over all rows of the CTA: number n is in place n % places; `full` completes a phase with each
-// copy, `empty` with the last warp that is done with it.
-template <class T, int NT>
-struct Ring {
-  using Part = RowPart<T, NT>;
-  static constexpr int VEC = Part::VEC;
-  uint4* slots;           // [places][NT]
+// A CTA's ring of units of STEP vectors of NT threads, and where one of its users is in it.  Units are numbered over all rows of the CTA: number
+// n is in place n % places; `full` completes a phase with each copy, `empty` with the last of the NT / 32 warps that give it back.
+template <class T, int NT, int STEP>
+struct UnitRing {
+  static constexpr int VEC = 16 / (int)sizeof(T), UNIT = STEP * NT;  // elements of a vector; vectors of a unit
+  static constexpr uint32_t NONE = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;  // -inf
+  uint4* slots;            // [places][UNIT]
   uint64_t *full, *empty;  // [places]
   int* status;
   int places, vocab, rank, size;
-  int first_it, first_place;  // the oldest block that is still needed of the row that is worked on, and its place
-  uint32_t first_phase;
-  const T* z;
-  size_t ld, rows, row_step;
+  int place = 0;  // of the unit that comes next, and its phase
+  uint32_t phase = 0;
+  // of the row that is worked on: this CTA's units
+  const T* row;
+  int align, n_vec, n_units;
 
-  // By all threads of the CTA, the warp that copies among them; it sets up the barriers of `exchange` too.
-  __device__ __forceinline__ Ring(uint4* slots_, uint64_t* bars, int places_, int* status_, const T* z_, size_t ld_, size_t rows_, int vocab_, Exchange& exchange)
-      : slots(slots_), full(bars), empty(bars + VR_MAX_BLOCKS), status(status_), places(places_), vocab(vocab_), rank((int)cluster_ctarank()),
-        size((int)cluster_size()), first_it(0), first_place(0), first_phase(0), z(z_), ld(ld_), rows(rows_) {
-    row_step = gridDim.x / (unsigned)size;
-    exchange.bars = bars + 2 * VR_MAX_BLOCKS;
-    exchange.status = status;
+  // The barriers are set up by all threads of the CTA, which then meet.
+  __device__ __forceinline__ UnitRing(uint4* slots_, uint64_t* bars, int places_, int* status_, int vocab_)
+      : slots(slots_), full(bars), empty(bars + VR_MAX_UNITS), status(status_), places(places_), vocab(vocab_), rank((int)cluster_ctarank()),
+        size((int)cluster_size()) {
     for (int i = threadIdx.x; i < places; i += NT) {
       mbar_init(full + i, 1);
       mbar_init(empty + i, NT / 32);
     }
-    if (threadIdx.x < 2) mbar_init(exchange.bars + threadIdx.x, 1);
     mbar_fence_init();
     fence_proxy_async_smem();
-    cluster_sync_all();  // nobody sends to a CTA that does not run yet
   }
-  __device__ __forceinline__ Part part(size_t r) const { return Part(z + r * ld, vocab, rank, size); }
-  // The copies of all rows, in one thread of the warp that does nothing else.
-  __device__ __forceinline__ void copy_rows() const {
-    int place = 0;
-    uint32_t phase = 1;  // of `empty`: at first every place is
+  __device__ __forceinline__ void begin(const T* row_) {
+    row = row_;
+    align = (int)(((uintptr_t)row & 15) / sizeof(T));
+    n_vec = (align + vocab + VEC - 1) / VEC;
+    const int units = (n_vec + UNIT - 1) / UNIT;
+    n_units = (int)((unsigned)(units - rank + size - 1) / (unsigned)size);
+  }
+  __device__ __forceinline__ int first_vector(int u) const { return (u * size + rank) * UNIT; }
+  // the column of the first element of vector `i` of a unit
+  __device__ __forceinline__ int column_of(int u, int i) const { return (first_vector(u) + i) * VEC - align; }
+  __device__ __forceinline__ void next() {
+    if (++place == places) place = 0, phase ^= 1;
+  }
+  __device__ __forceinline__ uint4* unit() const { return slots + place * UNIT; }
+  __device__ __forceinline__ void wait() const { row_wait(full + place, phase, status); }
+  // the warp gives the unit back; what it wrote there comes before the copies that follow by the writers' fence
+  __device__ __forceinline__ void release() const {
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(empty + place);
+  }
+  __device__ __forceinline__ void copy_rows(const T* z, size_t ld, size_t rows, size_t row_step) {
     for (size_t r = cluster_id(); r < rows; r += row_step) {
-      const Part p = part(r);
-      const int first_whole = p.phase ? 1 : 0, end_whole = (p.phase + vocab) / VEC;  // vectors that lie in the row
-      for (int it = 0; it < p.n_it; ++it) {
-        const int first = p.first_vector(it), v0 = max(first, first_whole), v1 = min(first + NT, end_whole);
+      begin(z + r * ld);
+      for (int u = 0; u < n_units; ++u, next()) {
+        const int first = first_vector(u), v0 = max(first, align ? 1 : 0), v1 = min(first + UNIT, (align + vocab) / VEC);  // vectors that lie in the row
         const uint32_t bytes = v1 > v0 ? (uint32_t)(v1 - v0) * 16 : 0;
-        row_wait(empty + place, phase, status);
+        row_wait(empty + place, phase ^ 1, status);
         mbar_expect_tx(full + place, bytes);
-        if (bytes) bulk_load_1d(slots + place * NT + (v0 - first), p.row + (v0 * VEC - p.phase), bytes, full + place);
-        if (++place == places) place = 0, phase ^= 1;
+        if (bytes) bulk_load_1d(unit() + (v0 - first), row + (v0 * VEC - align), bytes, full + place);
       }
     }
   }
-  // n blocks of the row are done with, and perhaps the row is
-  __device__ __forceinline__ void advance(int n, bool next_row_begins) {
-    first_it = next_row_begins ? 0 : first_it + n;
-    first_place += n;
-    if (first_place >= places) first_place -= places, first_phase ^= 1;
-  }
-  __device__ __forceinline__ int place(int it) const {
-    const int n = first_place + it - first_it;
-    return n < places ? n : n - places;
-  }
-  __device__ __forceinline__ uint4* block(int it) const { return slots + place(it) * NT; }
-  __device__ __forceinline__ void wait(int it) const {
-    const int n = first_place + it - first_it;
-    row_wait(full + (n < places ? n : n - places), first_phase ^ (n < places ? 0u : 1u), status);
-  }
-  // The warp is done with n blocks that lie side by side, and what it wrote there comes before the copies that follow (the writers' fence).
-  __device__ __forceinline__ void release(const uint4* first, int n) const {
-    __syncwarp();
-    const int lane = threadIdx.x & 31;
-    if (lane < n) mbar_arrive(empty + (int)(first - slots) / NT + lane);
-  }
-  // The warp is done with the row.
-  __device__ __forceinline__ void release_all(const Part& p) const {
-    __syncwarp();
-    for (int it = threadIdx.x & 31; it < p.n_it; it += 32) mbar_arrive(empty + place(it));
-  }
-  // What no copy brings of a block: vectors that stick out of the row, element by element, and -inf behind the row's last one, by the
-  // threads that they belong to.
-  __device__ __forceinline__ void complete(const Part& p, int it) const {
-    const int v = p.first_vector(it) + (int)threadIdx.x, c = v * VEC - p.phase;
+  // What no copy brings of the vector `i` of a unit: one that sticks out of the row, element by element, and -inf behind the row's last one.
+  __device__ __forceinline__ void complete_vector(int u, int i, uint4* slot) const {
+    const int c = column_of(u, i);
     if (c >= 0 && c + VEC <= vocab) return;
-    uint4* slot = block(it) + threadIdx.x;
-    if (v >= p.n_vec) {
-      *slot = make_uint4(Part::NONE, Part::NONE, Part::NONE, Part::NONE);
+    if (c >= vocab) {
+      *slot = make_uint4(NONE, NONE, NONE, NONE);
     } else {
       alignas(16) T e[VEC];
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) e[i] = c + i >= 0 && c + i < vocab ? p.row[c + i] : from_f32<T>(-INFINITY);
+      for (int k = 0; k < VEC; ++k) e[k] = c + k >= 0 && c + k < vocab ? row[c + k] : from_f32<T>(-INFINITY);
       *slot = *(const uint4*)e;
     }
   }
-  // The whole row is there, for every thread behind the next barrier of the CTA: each warp waits for a few blocks.
-  __device__ __forceinline__ void wait_all(const Part& p) const {
-    for (int it = threadIdx.x / 32; it < p.n_it; it += NT / 32) wait(it);
-    if (p.n_it > 0) complete(p, 0);
-    if (p.n_it > 1) complete(p, p.n_it - 1);
-  }
-  // f(block, blocks, where the thread's vector of the first lies) for the one or two runs of places that hold the row.
-  template <class F>
-  __device__ __forceinline__ void runs(const Part& p, F&& f) const {
-    const int n = min(p.n_it, places - first_place);
-    f(0, n, slots + first_place * NT + threadIdx.x);
-    if (n < p.n_it) f(n, p.n_it - n, slots + threadIdx.x);
-  }
-  static constexpr int GROUP = 4;
-  // The thread's reference for exponentials, one of its elements or -inf, and the sum of its exponentials relative to it.  The reference
-  // is the largest of the first vectors: an exponential may be as large as 2^60 before it changes, so that it rarely does.  KEEP
-  // (32-bit rows): the exponentials take their elements' place.
-  template <bool KEEP>
-  __device__ __forceinline__ float exponentials(const Part& p, const ExpT& ex, float* reference) const {
-    float ref = -INFINITY;
-    const float most = 60.0f / ex.hi;
-    F2 acc[4] = {0, 0, 0, 0};
-    auto work = [&](int it, uint4* at, auto count) {
-      constexpr int N = decltype(count)::value;
-      uint4 v[N];
-#pragma unroll
-      for (int j = 0; j < N; ++j) v[j] = at[j * NT];
-      float top;
-      if constexpr (sizeof(T) == 4) {
-        top = max_nan(__uint_as_float(v[0].x), __uint_as_float(v[0].y), max_nan(__uint_as_float(v[0].z), __uint_as_float(v[0].w)));
-#pragma unroll
-        for (int j = 1; j < N; ++j) top = max_nan(max_nan(top, __uint_as_float(v[j].x), __uint_as_float(v[j].y)), __uint_as_float(v[j].z), __uint_as_float(v[j].w));
-      } else {
-        using T2 = std::conditional_t<std::is_same<T, __half>::value, __half2, __nv_bfloat162>;
-        T2 m = __hmax2_nan(__hmax2_nan(*(const T2*)&v[0].x, *(const T2*)&v[0].y), __hmax2_nan(*(const T2*)&v[0].z, *(const T2*)&v[0].w));
-#pragma unroll
-        for (int j = 1; j < N; ++j)
-          m = __hmax2_nan(m, __hmax2_nan(__hmax2_nan(*(const T2*)&v[j].x, *(const T2*)&v[j].y), __hmax2_nan(*(const T2*)&v[j].z, *(const T2*)&v[j].w)));
-        top = max_nan(to_f32(m.x), to_f32(m.y));
-      }
-      if (!(top <= ref + most) && ref == ref) {  // the first finite ones, ones that are far larger, a NaN, which stays
-        if (ref > -INFINITY) {
-          const float by = ex(ref - top);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) acc[j] = mul2(acc[j], pack2(by, by));
-          if constexpr (KEEP) {
+  // the thread's vectors of a unit, the first of which is at `at`
+  __device__ __forceinline__ void complete(int u, uint4* at) const {
 #pragma unroll 1
-            for (int i = 0; i < it; ++i) {
-              float4* e = (float4*)(block(i) + threadIdx.x);
-              *e = make_float4(e->x * by, e->y * by, e->z * by, e->w * by);
-            }
-          }
-        }
-        ref = top;
-      }
-      const float r = ref > -INFINITY ? ref : 0.0f;
-      const F2 minus_ref = pack2(-r, -r);
-#pragma unroll
-      for (int j = 0; j < N; ++j) {
-        float x[VEC];
-        Part::unpack(v[j], x);
-#pragma unroll
-        for (int i = 0; i < VEC; i += 2) {
-          ex.pair(pack2(x[i], x[i + 1]), minus_ref, x + i, x + i + 1);
-          acc[(j * VEC + i) / 2 & 3] = add2(acc[(j * VEC + i) / 2 & 3], pack2(x[i], x[i + 1]));
-        }
-        if constexpr (KEEP) at[j * NT] = make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
-      }
-    };
-    runs(p, [&](int it, int n, uint4* at) {
-#pragma unroll 1
-      for (; n >= GROUP; n -= GROUP, it += GROUP, at += GROUP * NT) work(it, at, std::integral_constant<int, GROUP>());
-#pragma unroll 1
-      for (; n > 0; --n, ++it, at += NT) work(it, at, std::integral_constant<int, 1>());
-    });
-    *reference = ref;
-    float a, b;
-    unpack2(add2(add2(acc[0], acc[1]), add2(acc[2], acc[3])), &a, &b);
-    return a + b;
+    for (int j = 0; j < STEP; ++j) complete_vector(u, j * NT + (int)threadIdx.x % NT, at + j * NT);
   }
-  // What f(vector, its VEC results) makes of every vector of the thread goes into the row `out`, and the blocks are released on the way.
-  template <class O, class F>
-  __device__ __forceinline__ void put(const Part& p, O* out, F&& f) {
-    const bool aligned = ((uintptr_t)out - (uintptr_t)p.phase * sizeof(O)) % (VEC * sizeof(O) < 16 ? VEC * sizeof(O) : 16) == 0;
-    const int stride = p.size * NT * VEC;  // columns from block to block
-    runs(p, [&](int it, int n, const uint4* at) {
-#pragma unroll 1
-      for (int end = it + n; it < end; it += GROUP, at += GROUP * NT) {
-        const int c = p.column(it), left = min(GROUP, end - it);
-        if (aligned && left == GROUP && it > 0 && it + GROUP < p.n_it) {
-          uint4 v[GROUP];
-          O* to = out + c;
-#pragma unroll
-          for (int j = 0; j < GROUP; ++j) v[j] = at[j * NT];
-#pragma unroll
-          for (int j = 0; j < GROUP; ++j, to += stride) {
-            float x[VEC];
-            f(v[j], x);
-            put_vector<O, VEC>(to, x);
-          }
-        } else {
-#pragma unroll 1
-          for (int j = 0; j < left; ++j) {
-            float x[VEC];
-            f(at[j * NT], x);
-            const int cj = c + j * stride;
-            if (aligned && cj >= 0 && cj + VEC <= vocab) put_vector<O, VEC>(out + cj, x);
-            else put_elements<O, VEC>(out, cj, vocab, x);
-          }
-        }
-        release(at, left);
-      }
-    });
-  }
-  // The results e f, e the exponentials relative to the row's reference (-inf: all are 0); `mine` is the thread's.
-  template <class O>
-  __device__ __forceinline__ void put_exponentials(const Part& p, O* out, float mine, float reference, float f, const ExpT& ex) {
-    if constexpr (sizeof(T) == 4) {  // they are there, relative to the thread's
-      const float by = mine > -INFINITY ? ex(mine - reference) * f : f;
-      put(p, out, [&](const uint4& v, float* x) {
-        Part::unpack(v, x);
-#pragma unroll
-        for (int i = 0; i < VEC; i += 2) unpack2(mul2(pack2(x[i], x[i + 1]), pack2(by, by)), x + i, x + i + 1);
-      });
-    } else {
-      const float ref = reference > -INFINITY ? reference : 0.0f;
-      const F2 minus_ref = pack2(-ref, -ref), by = pack2(f, f);
-      put(p, out, [&](const uint4& v, float* x) {
-        Part::unpack(v, x);
-#pragma unroll
-        for (int i = 0; i < VEC; i += 2) {
-          ex.pair(pack2(x[i], x[i + 1]), minus_ref, x + i, x + i + 1);
-          unpack2(mul2(pack2(x[i], x[i + 1]), by), x + i, x + i + 1);
-        }
-      });
-    }
-  }
+  // the column of the first element of the thread's j-th vector of a unit
+  __device__ __forceinline__ int column(int u, int j) const { return column_of(u, j * NT + (int)threadIdx.x % NT); }
 };
 
 // The warp's sum of its threads' exponentials, relative to the largest of their references.  In 32 bits: five roundings, which differ from
@@ -536,26 +350,6 @@ __device__ __forceinline__ double lane_join(int n, F&& get, const ExpT& ex, floa
   return s;
 }
 
-// How rows are held.  Threads that work: 256 where two CTAs with a row (or its part) each find room on an SM, else 512.  The CTAs of a row's
-// cluster: as few as have room for it, more where there are so few rows that SMs would be idle.  The ring's blocks: all that fit
-// beside `other` bytes, as far as there are rows to fill them.
-struct RowShape {
-  int threads, cluster, places;
-  size_t smem;
-};
-inline RowShape row_shape(const rt_ctx* c, size_t rows, int vocab, int dtype, size_t other) {
-  const int vec = dtype == RT_DT_F32 ? 4 : 8, vectors = (vec - 1 + vocab + vec - 1) / vec;  // at the worst alignment
-  const size_t third = 68 * 1024, half = 104 * 1024, all = VR_MOST_SMEM;
-  int size = 1;
-  while (size * 2 <= VR_MAX_CLUSTER && vectors > 512 * size && rows * size * 2 <= (size_t)c->num_sms) size *= 2;
-  auto need = [&](int threads) { return (size_t)(((vectors + threads - 1) / threads + size - 1) / size) * threads * 16 + other; };
-  while (size < VR_MAX_CLUSTER && need(512) > all) ++size;
-  const int threads = need(256) <= half ? 256 : 512;
-  const size_t block = (size_t)threads * 16, room = need(threads) <= third ? third : need(threads) <= half ? half : all;
-  const size_t turns = (rows * size + c->num_sms - 1) / c->num_sms, each = (need(threads) - other) / block;
-  const size_t places = std::max(each, std::min(std::min((room - other) / block, (size_t)VR_MAX_BLOCKS), each * std::min(turns, (size_t)4)));
-  return {threads, size, (int)places, places * block + other};
-}
 // Calls f with the number of threads that work as a constant.
 template <class F>
 inline int with_threads(int threads, F&& f) {
@@ -581,7 +375,7 @@ inline int launch_clusters(rt_ctx* c, void (*kernel)(KArgs...), bool stay, size_
   cfg.attrs = at;
   cfg.numAttrs = 1;
   if (stay) {
-    int& most = c->clusters_at_once[std::make_tuple((const void*)kernel, size, smem)];
+    int& most = c->clusters_at_once[std::make_tuple((const void*)kernel, size * 1024 + threads, smem)];
     if (most == 0 && (cudaOccupancyMaxActiveClusters(&most, kernel, &cfg) != cudaSuccess || most < 1)) return 3;
     const size_t turns = (rows + most - 1) / most;
     cfg.gridDim = dim3((unsigned)((rows + turns - 1) / turns * size));
