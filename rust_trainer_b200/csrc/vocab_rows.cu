@@ -118,9 +118,14 @@ __device__ __forceinline__ void write_row(UnitRing<T, NT, ROW_STEP>& ring, O* ou
   constexpr int VEC = Ring::VEC;
   const bool aligned = ((uintptr_t)out - (uintptr_t)ring.align * sizeof(O)) % (VEC * sizeof(O) < 16 ? VEC * sizeof(O) : 16) == 0;
   const float ref = reference > -INFINITY ? reference : 0.0f;
-  // in two factors: what is left of an exponential of 2^30 may be 2^30 larger than what one factor can say
-  const float h = sizeof(T) == 4 && mine > -INFINITY ? ex(0.5f * (mine - reference)) : 1.0f;
-  f *= h;
+  // far below the reference in two factors: what is left of an exponential of 2^30 may be 2^30 larger than what one factor can say
+  float h = 1.0f;
+  if (sizeof(T) == 4 && mine > -INFINITY) {
+    const bool far = (mine - reference) * ex.hi < -60.0f;
+    const float by = ex(far ? 0.5f * (mine - reference) : mine - reference);
+    if (far) h = by;
+    f *= by;
+  }
   const F2 minus_ref = pack2(-ref, -ref), by = pack2(f, f), half_way = pack2(h, h);
 #pragma unroll 1
   for (int u = 0; u < ring.n_units; ++u) {
@@ -148,6 +153,32 @@ __device__ __forceinline__ void write_row(UnitRing<T, NT, ROW_STEP>& ring, O* ou
   }
 }
 
+// The lane's part of the sum of all warps' exponentials, relative to the largest of their references.
+template <int WARPS>
+__device__ __forceinline__ float join_stats(const RowStat* stat, int size, const ExpT& ex, float* m) {
+  constexpr int EACH = VR_MAX_CLUSTER * WARPS / 32;
+  RowStat mine[EACH];
+  float top = -INFINITY, s = 0.0f;
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    const int w = i * 32 + (threadIdx.x & 31);
+    mine[i] = w < size * WARPS ? stat[w] : RowStat{-INFINITY, 0.0f};
+    top = max_nan(top, mine[i].m);
+  }
+  *m = warp_max_nan(top);
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) s += mine[i].m > -INFINITY ? mine[i].s * ex(mine[i].m - *m) : 0.0f;
+  return s;
+}
+__device__ __forceinline__ float2 warp_sum_f32x2(float a, float b) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    a += __shfl_xor_sync(0xffffffffu, a, o);
+    b += __shfl_xor_sync(0xffffffffu, b, o);
+  }
+  return make_float2(a, b);
+}
+
 template <class T, class O, int NT>
 __global__ void __maxnreg__(NT == 256 ? 96 : 72)
 softmax_rows_kernel(const T* z, size_t ld, size_t rows, int vocab, ExpT ex, O* prob, size_t prob_ld, int places, int* status) {
@@ -166,9 +197,8 @@ softmax_rows_kernel(const T* z, size_t ld, size_t rows, int vocab, ExpT ex, O* p
   mbar_fence_init();
   cluster_sync_all();  // nobody sends to a CTA that does not run yet
   const size_t row_step = gridDim.x / (unsigned)ring.size;
-  const int warps = ring.size * WARPS;
   if (tid < NT) {
-    sum_rows<T, NT, sizeof(T) == 4>(ring, z, ld, rows, row_step, ex, b, refs, stats, warps * sizeof(RowStat), false, false);
+    sum_rows<T, NT, sizeof(T) == 4>(ring, z, ld, rows, row_step, ex, b, refs, stats, ring.size * WARPS * sizeof(RowStat), false, false);
   } else if (tid < 2 * NT) {
     uint32_t i = 0;
     for (size_t r = cluster_id(); r < rows; r += row_step, ++i) {
@@ -176,7 +206,7 @@ softmax_rows_kernel(const T* z, size_t ld, size_t rows, int vocab, ExpT ex, O* p
       row_wait_turn(b.exchange, i, 2, status);
       const RowStat* stat = stats[i & 3];
       float m;
-      const float sum = (float)warp_sum_f64(lane_join(warps, [&](int w, float* mi, float* si) { *mi = stat[w].m, *si = stat[w].s; }, ex, &m));
+      const float sum = warp_sum_f32(join_stats<WARPS>(stat, ring.size, ex, &m));
       // a row of -inf has no probabilities, one with a NaN or +inf no number for them
       const float f = m == -INFINITY ? 0.0f : m < INFINITY ? 1.0f / sum : NAN;
       row_wait_turn(b.summed, i, 1, status);
@@ -194,33 +224,32 @@ softmax_rows_kernel(const T* z, size_t ld, size_t rows, int vocab, ExpT ex, O* p
 struct alignas(16) ListStat {
   double listed;
   float rest, by;
-  float top, unused[3];
+  float top, listed32, unused[2];
   static constexpr int SENT = 24;
 };
 struct alignas(16) LossStat {  // the teacher's mass, and sum q (t_j - z_j / T), the z relative to the largest
   double mass, cross;
 };
-// What a row's sums make of it: a gradient outside of the list is exp(z - reference) outside, one on it e listed - q by, e relative to the largest listed.
+// What a row's sums make of it: a gradient outside of the list is exp(z - reference) outside, one on it e listed - q by, e relative to the largest
+// listed.  (Few instructions: run once a row between loops that do not leave them in the caches, each line of them is waited for.)
 struct RowGradient {
   float reference, outside, listed, by;
   bool idle;
 };
 template <int WARPS>
-__device__ __forceinline__ RowGradient row_gradient(const RowStat* stat, const ListStat* list, int size, float w, float t, bool scaled, const ExpT& ex) {
+__device__ __forceinline__ RowGradient row_gradient(const RowStat* stat, const ListStat* list, int size, bool idle, float factor, const ExpT& ex) {
   RowGradient g;
-  float mo, on = 0.0f;
-  float so = (float)lane_join(size * WARPS, [&](int i, float* mi, float* si) { *mi = stat[i].m, *si = stat[i].s; }, ex, &mo);
-  so = warp_sum_f32(so);
-  for (int i = 0; i < size; ++i) on += (float)list[i].listed;
-  const float top = list[0].top, rest = list[0].rest, m = max_nan(mo, top), by = scaled ? 1.0f : w / t;
-  const bool bad = !(m < INFINITY);
+  float mo;
+  const int lane = threadIdx.x & 31;
+  const float2 sums = warp_sum_f32x2(join_stats<WARPS>(stat, size, ex, &mo), lane < size ? list[lane].listed32 : 0.0f);
+  const float so = sums.x, on = sums.y, top = list[0].top, rest = list[0].rest, m = max_nan(mo, top);
   const float rest_to = mo > -INFINITY ? ex(mo - m) : 0.0f, top_to = top > -INFINITY ? ex(top - m) : 0.0f;
-  const float inv = 1.0f / (so * rest_to + on * top_to);
+  const float scale = m < INFINITY ? factor : NAN, inv = scale / (so * rest_to + on * top_to);
   g.reference = mo;
-  g.outside = bad ? NAN : so > 0.0f ? (rest_to * inv - rest / so) * by : 0.0f;
-  g.listed = bad ? NAN : m > -INFINITY ? top_to * inv * by : 0.0f;
-  g.by = list[0].by * by;
-  g.idle = w == 0.0f || rest < 0.0f;
+  g.outside = so > 0.0f ? rest_to * inv - rest / so * scale : scale * 0.0f;
+  g.listed = m > -INFINITY ? top_to * inv : scale * 0.0f;
+  g.by = list[0].by * factor;
+  g.idle = idle || rest < 0.0f;
   return g;
 }
 
@@ -271,18 +300,18 @@ distill_rows_kernel(const T* z, size_t ld, size_t rows, int vocab, float t, ExpT
   mbar_fence_init();
   cluster_sync_all();  // nobody sends to a CTA that does not run yet
   const size_t row_step = gridDim.x / (unsigned)ring.size;
-  const int warps = ring.size * WARPS, writers = d ? NT : 0, copier = NT + writers, finisher = copier + 32, lister = finisher + 32;
+  const int writers = d ? NT : 0, copier = NT + writers, finisher = copier + 32, lister = finisher + 32;
   if (tid < NT) {
-    const uint32_t bytes = warps * sizeof(RowStat) + ring.size * ListStat::SENT + (finds_loss ? sizeof(LossStat) : 0);
+    const uint32_t bytes = ring.size * WARPS * sizeof(RowStat) + ring.size * ListStat::SENT + (finds_loss ? sizeof(LossStat) : 0);
     if (d) sum_rows<T, NT, sizeof(T) == 4>(ring, z, ld, rows, row_step, ex, b, refs, stats, bytes, true, false);
     else sum_rows<T, NT, false>(ring, z, ld, rows, row_step, ex, b, refs, stats, bytes, true, true);
   } else if (tid < copier) {  // writes
     uint32_t i = 0;
     for (size_t r = cluster_id(); r < rows; r += row_step, ++i) {
-      const float w = weight ? weight[r] : 1.0f;
+      const float w = weight ? weight[r] : 1.0f, factor = row_scale ? 1.0f : w / t;
       ring.begin(z + r * ld);
       row_wait_turn(b.exchange, i, 2, status);
-      const RowGradient g = row_gradient<WARPS>(stats[i & 3], lists[i & 3], ring.size, w, t, row_scale != nullptr, ex);
+      const RowGradient g = row_gradient<WARPS>(stats[i & 3], lists[i & 3], ring.size, w == 0.0f, factor, ex);
       row_wait_turn(b.summed, i, 1, status);
       // (rows that nothing is learnt from, whatever their logits are, have zeros)
       if (!g.idle) {
@@ -311,8 +340,7 @@ distill_rows_kernel(const T* z, size_t ld, size_t rows, int vocab, float t, ExpT
         const double mass = losses[i & 3].mass, cross = losses[i & 3].cross;
         const float top = list[0].top;
         float mo;
-        double so = lane_join(warps, [&](int w, float* mi, float* si) { *mi = stat[w].m, *si = stat[w].s; }, ex, &mo), on = 0.0;
-        so = warp_sum_f64(so);
+        double so = warp_sum_f64(join_stats<WARPS>(stat, ring.size, ex, &mo)), on = 0.0;
         for (int c = 0; c < ring.size; ++c) on += list[c].listed;
         const double rest = tail ? fmax(0.0, 1.0 - mass) : 0.0;
         // log(on + outside), the first relative to `top`, the second to mo, log(outside), log(rest) and log(mass): side by side
@@ -330,7 +358,7 @@ distill_rows_kernel(const T* z, size_t ld, size_t rows, int vocab, float t, ExpT
         }
       }
       if (d) {
-        const RowGradient g = row_gradient<WARPS>(stat, list, ring.size, w, t, row_scale != nullptr, ex);
+        const RowGradient g = row_gradient<WARPS>(stat, list, ring.size, w == 0.0f, row_scale ? 1.0f : w / t, ex);
         row_wait_turn(b.written, i, 1, status);
         for (int j = lane; j < k; j += 32) {
           const int c = s_mine[i & 1][j];
@@ -455,7 +483,7 @@ distill_rows_kernel(const T* z, size_t ld, size_t rows, int vocab, float t, ExpT
         if (lane < ring.size) {
           const uint32_t to = mapa_u32(smem_u32(&lists[i & 3][ring.rank]), lane), its_bar = mapa_u32(smem_u32(bar), lane);
           send(to, its_bar, (uint32_t)__double2loint(on), (uint32_t)__double2hiint(on), __float_as_uint(rest), __float_as_uint(by));
-          send(to + 16, its_bar, __float_as_uint(top), 0u);
+          send(to + 16, its_bar, __float_as_uint(top), __float_as_uint((float)on));
         }
         if (finds_loss && lane == 0)
           send(mapa_u32(smem_u32(&losses[i & 3]), 0), mapa_u32(smem_u32(bar), 0), (uint32_t)__double2loint(mass), (uint32_t)__double2hiint(mass),

@@ -330,26 +330,6 @@ __device__ __forceinline__ float warp_sum_f32(float v) {
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
-// The row's sum from n warps' references and sums (none: -inf, 0), as get(i, &m, &s) gives them: the lane's part of it, relative to *m.
-template <class F>
-__device__ __forceinline__ double lane_join(int n, F&& get, const ExpT& ex, float* m) {
-  float mi[4], si[4], top = -INFINITY;  // at most 128 warps
-  const int lane = threadIdx.x & 31;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    mi[i] = -INFINITY;
-    si[i] = 0.0f;
-    if (i * 32 + lane < n) get(i * 32 + lane, mi + i, si + i);
-    top = max_nan(top, mi[i]);
-  }
-  *m = warp_max_nan(top);
-  double s = 0.0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (i * 32 < n && mi[i] > -INFINITY) s += (double)(si[i] * ex(mi[i] - *m));
-  return s;
-}
-
 // Calls f with the number of threads that work as a constant.
 template <class F>
 inline int with_threads(int threads, F&& f) {
