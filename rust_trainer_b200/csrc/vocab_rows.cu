@@ -156,7 +156,7 @@ __device__ __forceinline__ void write_row(UnitRing<T, NT, ROW_STEP>& ring, O* ou
 // The lane's part of the sum of all warps' exponentials, relative to the largest of their references.
 template <int WARPS>
 __device__ __forceinline__ float join_stats(const RowStat* stat, int size, const ExpT& ex, float* m) {
-  constexpr int EACH = VR_MAX_CLUSTER * WARPS / 32;
+  constexpr int EACH = (VR_MAX_CLUSTER * WARPS + 31) / 32;
   RowStat mine[EACH];
   float top = -INFINITY, s = 0.0f;
 #pragma unroll
@@ -496,28 +496,34 @@ distill_rows_kernel(const T* z, size_t ld, size_t rows, int vocab, float t, ExpT
   }
 }
 
-// How rows are held.  Threads that sum, and that write: 128 where that is no more than eight units of a row, else 256.  The CTAs of a row's cluster: as
-// few as hold two rows, one that is summed and one that is written (longer rows have eight and are held once, at least), more where there are so few
-// rows that SMs would be idle.  The ring's units: all that fit, as far as there are rows to fill them.
+// How rows are held.  Threads that sum, and that write: few for short rows, of which an SM then holds several (registers admit five CTAs of 64
+// threads, two of 128 or one of 256).  Distillation from 32 entries, by threads and the ring's KB:
+//   4096 rows of 640 f32   64 x 32: 33 us, 128 x 66: 49, 256 x 208: 94
+//   4096 of 2500 f32       64 x 32: 41, 128 x 66: 55, 256 x 208: 100
+//   4096 of 8000 f32       128 x 66: 68, 256 x 208: 102       2048 of them: 64 x 32: 49, 128 x 66: 41
+//   4096 of 16000 f32      128 x 66: 147, 256 x 208: 109
+// The CTAs of a row's cluster: as few as hold two rows, one that is summed and one that is written (longer rows have eight and are held once, at
+// least); 1024 rows of 151936 f32 took 238 us with six CTAs, 272 with eight and 330 with four, 2048 of 128256 bf16 268 with three, 287 with two
+// and 303 with four.  More where there are so few rows that SMs would be idle.  The ring's units: all that fit, as far as there are rows to fill them.
 struct RowShape {
   int threads, cluster, places;
   size_t smem;
 };
 static RowShape row_shape(const rt_ctx* c, size_t rows, int vocab, int dtype) {
   const int vec = dtype == RT_DT_F32 ? 4 : 8, vectors = (vec - 1 + vocab + vec - 1) / vec;  // at the worst alignment
-  const int threads = vectors <= 2048 ? 128 : 256, units = (vectors + ROW_STEP * threads - 1) / (ROW_STEP * threads);
-  const size_t unit = (size_t)ROW_STEP * threads * 16, third = 66 * 1024, half = 100 * 1024, all = VR_MOST_SMEM;
+  const int threads = vectors <= 768 ? 64 : vectors <= 2048 ? 128 : 256, units = (vectors + ROW_STEP * threads - 1) / (ROW_STEP * threads);
+  const size_t unit = (size_t)ROW_STEP * threads * 16, room = threads == 64 ? 32 * 1024 : threads == 128 ? 66 * 1024 : VR_MOST_SMEM;
   int size = 1;
   while (size * 2 <= VR_MAX_CLUSTER && units > size && rows * size * 2 <= (size_t)c->num_sms) size *= 2;
   auto each = [&] { return (size_t)((units + size - 1) / size); };
-  while (size < VR_MAX_CLUSTER && 2 * each() * unit > all) ++size;
+  while (size < VR_MAX_CLUSTER && 2 * each() * unit > room) ++size;
   const size_t turns = (rows * size + c->num_sms - 1) / c->num_sms, want = each() * std::min(turns, (size_t)4);
-  const size_t room = 2 * each() * unit <= third ? third : 2 * each() * unit <= half ? half : all;
   const size_t places = std::max(each(), std::min(std::min(room / unit, (size_t)VR_MAX_UNITS), want));
   return {threads, size, (int)places, places * unit};
 }
 template <class F>
 static int with_row_threads(int threads, F&& f) {
+  if (threads == 64) return f(std::integral_constant<int, 64>());
   if (threads == 128) return f(std::integral_constant<int, 128>());
   return f(std::integral_constant<int, 256>());
 }
