@@ -79,7 +79,8 @@ struct RunningSum {
   }
 };
 
-template <class T, int NT>
+// SHORT: rows of one unit, where not all threads may hold elements; what such rows need took 3 to 5 % of long ones' time.
+template <class T, int NT, bool SHORT>
 __global__ void __launch_bounds__(NT + 32, ctas_of(NT))
 top_logits_kernel(const T* z, size_t ld, size_t rows, int vocab, float t, ExpT ex, int k, int* index, float* logp, float* lse, int places,
                   int kept_most, int room_most, int* status) {
@@ -107,31 +108,33 @@ top_logits_kernel(const T* z, size_t ld, size_t rows, int vocab, float t, ExpT e
   const double inv_t = 1.0 / t;
   const float hi = ex.hi;
   // values of a warp in the sample: W warps send at most W + k + W of them
-  const int each = min((k + WARPS - 1) / WARPS + 1, 32), warps = ring.size * WARPS;
+  const int each_of_all = min((k + WARPS - 1) / WARPS + 1, 32), warps = ring.size * WARPS;
+  int holders = WARPS, each = each_of_all, sampled = WARPS * each;  // warps that hold elements of the row
   TopKey *kept = (TopKey*)slots, *room = kept + kept_most;
   const int room_each = room_most / ring.size;
   // A value that k of the threads' maxima reach, and not many more of the sample's, in every warp the same.
   auto bound_of = [&](float largest) {
     const uint32_t sorted = warp_sort(order32(largest));
     work_sync<NT>();  // the last one's sample has been read
-    if (lane < each) sample[warp * each + lane] = sorted;
+    if (lane < each && (!SHORT || warp < holders)) sample[warp * each + lane] = sorted;
     work_sync<NT>();
     uint32_t some[SAMPLE_LANE], lo = 0xffffffffu, hi = 0;  // lo is reached by k; no value is above hi
 #pragma unroll
     for (int i = 0; i < SAMPLE_LANE; ++i) {
-      const bool on = i * 32 + lane < WARPS * each;
+      const bool on = i * 32 + lane < sampled;
       some[i] = on ? sample[i * 32 + lane] : 0;
       if (on) lo = min(lo, some[i]);
       hi = max(hi, some[i]);
     }
     lo = __reduce_min_sync(0xffffffffu, lo);
     hi = __reduce_max_sync(0xffffffffu, hi);
+    if (SHORT && sampled < k) return order32(-INFINITY);  // too few threads hold elements
     while (hi > lo) {  // at most 32 times
       const uint32_t mid = lo + (hi - lo) / 2 + 1;
       int n = 0;
 #pragma unroll
       for (int i = 0; i < SAMPLE_LANE; ++i)
-        if (i * 32 < WARPS * each) n += some[i] >= mid;
+        if (i * 32 < sampled) n += some[i] >= mid;
       n = __reduce_add_sync(0xffffffffu, n);
       if (n >= k) lo = mid;
       else hi = mid - 1;
@@ -149,6 +152,12 @@ top_logits_kernel(const T* z, size_t ld, size_t rows, int vocab, float t, ExpT e
   };
   for (size_t r = cluster_id(); r < rows; r += row_step) {
     ring.begin(z + r * ld);
+    if constexpr (SHORT) {
+      const int with = min(NT, ring.n_vec), whole = max(with / 32, 1);
+      holders = (with + 31) / 32;
+      each = min((k + whole - 1) / whole + 1, min(32, 32 * SAMPLE_LANE / holders));
+      sampled = holders * each;
+    }
     RunningSum sum;
     float largest = -INFINITY;  // of the thread's elements
     uint32_t bound = 0;
@@ -208,6 +217,13 @@ top_logits_kernel(const T* z, size_t ld, size_t rows, int vocab, float t, ExpT e
           f2.x = f2.y = f;
 #pragma unroll
           for (int i = 0; i < 8; ++i) hits |= (~__hlt2_mask(x2[i], f2) & 0x00010001u) << i;
+        }
+        if (SHORT && from == -INFINITY) {  // nothing is below: all of a short row, but not what lies outside of it
+#pragma unroll 1
+          for (int i = 0; i < 16; ++i) {
+            const int c = ring.column(s, i / VEC) + i % VEC;
+            if (c < 0 || c >= vocab) hits &= ~(1u << (sizeof(T) == 4 ? 15 - i : i / 2 + 16 * (i & 1)));
+          }
         }
         if (*(volatile int*)&s_kept <= kept_most) {  // else there are too many already
           int p = atomicAdd(&s_kept, __popc(hits));
@@ -332,7 +348,7 @@ top_logits_kernel(const T* z, size_t ld, size_t rows, int vocab, float t, ExpT e
       work_sync<NT>();
       found = tell((uint32_t)s_n, 0);
     }
-    const int n_mine = (int)found[ring.rank].x;
+    int n_mine = (int)found[ring.rank].x;
     if (ring.size > 1) {  // everybody's to everybody
       int n = 0;
       for (int i = 0; i < ring.size; ++i) n += (int)found[i].x;
@@ -346,6 +362,27 @@ top_logits_kernel(const T* z, size_t ld, size_t rows, int vocab, float t, ExpT e
       }
       exchange.wait();
     }
+    const TopKey* others_room = room;
+    // Many more than k, of a short row with a long list: ranks by counting would take the square of them.  A key that k reach, and few more.
+    if (SHORT && n_mine > 2 * k + 64) {
+      TopKey low = 0, high = (TopKey)1 << (32 + TOP_INDEX_BITS);
+      while (high - low > 1) {  // at most 51 times
+        const TopKey mid = low + (high - low) / 2;
+        int n = 0;
+        for (int i = 0; i < n_mine; i += NT) n += work_count<NT>(i + tid < n_mine && mine[i + tid] >= mid);
+        if (n >= k) low = mid;
+        else high = mid;
+        if (n >= k && n <= k + k / 2 + 8) break;
+      }
+      if (tid == 0) s_kept = 0;
+      work_sync<NT>();
+      for (int i = tid; i < n_mine; i += NT)
+        if (mine[i] >= low) kept[atomicAdd(&s_kept, 1)] = mine[i];
+      work_sync<NT>();
+      n_mine = s_kept;
+      mine = kept;
+      others_room = kept;
+    }
     const double row_lse = s_lse;
     if (lse && tid == 0 && ring.rank == 0) lse[r] = (float)row_lse;
     // a thread an element: its rank is the number of larger ones
@@ -354,7 +391,7 @@ top_logits_kernel(const T* z, size_t ld, size_t rows, int vocab, float t, ExpT e
       int rank = 0;
       for (int o = 0; o < ring.size; ++o) {
         const int n = ring.size > 1 ? s_found[o] : n_mine;
-        const TopKey* const others = room + o * room_each;
+        const TopKey* const others = others_room + o * room_each;
 #pragma unroll 8
         for (int j = 0; j < n; ++j) rank += others[j] > key;
       }
@@ -380,7 +417,8 @@ int launch_top_logits(rt_ctx* c, const VocabRows& z, size_t rows, int vocab, flo
   return with_dtype(z.dtype, [&](auto* zt) {
     return with_threads(threads, [&](auto n) {
       using T = std::remove_pointer_t<decltype(zt)>;
-      return launch_clusters(c, top_logits_kernel<T, decltype(n)::value>, true, rows, threads + 32, size, places * unit + other, (const T*)z.p, z.ld, rows, vocab,
+      constexpr int NT = decltype(n)::value;
+      return launch_clusters(c, units == 1 ? top_logits_kernel<T, NT, true> : top_logits_kernel<T, NT, false>, true, rows, threads + 32, size, places * unit + other, (const T*)z.p, z.ld, rows, vocab,
                              temperature, exp_t(temperature), k, index, logp, lse, places, room.kept, room.ranked, c->status_dev);
     });
   });

@@ -153,6 +153,20 @@ __device__ __forceinline__ void send(uint32_t to, uint32_t bar, double v) {
 template <int NT>
 __device__ __forceinline__ void work_sync() { asm volatile("bar.sync 1, %0;" ::"n"(NT) : "memory"); }
 
+// of how many of the threads `v` is true
+template <int NT>
+__device__ __forceinline__ int work_count(bool v) {
+  int n;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "bar.red.popc.u32 %0, 1, %2, p;\n\t}"
+      : "=r"(n)
+      : "r"((uint32_t)v), "n"(NT)
+      : "memory");
+  return n;
+}
+
 // Waits for a phase of a barrier, asleep for up to some microseconds at a time: a warp that polls takes instructions from those that work.
 // The matmul's wait gives up when another kernel has reported anything; here an index out of range in one row must not end the
 // others' waits, so that only the time limit does.
