@@ -219,10 +219,11 @@ rt_status rt_op_cross_entropy(rt_ctx* ctx, const float* logits_host, size_t rows
  *   - a probability below 2^-126 of the row's largest may come out as 0;
  *   - among equal values (the two zeros are equal) the lowest index comes first.
  * Rows are `ld` elements apart (ld >= vocab; what lies behind the vocabulary is neither read nor written),
- * their elements RT_DT_F32, RT_DT_BF16 or RT_DT_F16; any element-aligned address is taken.  Sums are held in
- * 32 bits within a thread and 64 beyond.  The device forms only launch on the ctx stream: they allocate
- * nothing, share no workspace and may be captured; what a kernel finds wrong (an index out of range) is
- * reported by the next rt_ctx_synchronize, like a wait that ran out.  The host forms take f32 rows. */
+ * their elements RT_DT_F32, RT_DT_BF16 or RT_DT_F16; any element-aligned address is taken.  Sums over a row are
+ * held in 32 bits within a warp, and from there in 64 for log-sum-exps and losses, in 32 for probabilities and
+ * gradients.  The device forms only launch on the ctx stream: they allocate no device memory, share no workspace
+ * and may be captured; what a kernel finds wrong (an index out of range) is reported by the next
+ * rt_ctx_synchronize, like a wait that ran out.  The host forms take f32 rows. */
 #define RT_TOP_MAX 256      /* entries of a teacher's list, at most */
 #define RT_VOCAB_MAX 393216 /* elements of a row, at most */
 /* What becomes of the probability that a teacher's list leaves out: the list is normalised to one, or the rest is one
@@ -259,8 +260,8 @@ rt_status rt_softmax_dev(rt_ctx* ctx, const void* logits_dev, int dtype, size_t 
  * the drafts were certain, q = 1).  With u = u_accept[draft] in [0, 1), a draft d stands if all before it stand and
  * u q(d) < p(d).  accepted[s] is how many do.  token[s] follows them: drawn with u_sample[s] in [0, 1) from
  * max(p - q, 0) at the first draft that does not stand (p without d, for certain drafts; p where nothing is left), or from
- * p of the last row: the lowest index at which the running sum exceeds u_sample times the whole sum.  Products and sums are
- * in 64 bits, so that 16-bit and 32-bit probabilities are compared exactly.  What is no finite positive number counts as
+ * p of the last row: the lowest index at which the running sum exceeds u_sample times the whole sum.  Products are in 64 bits, so
+ * that 16-bit and 32-bit probabilities are compared exactly; sums are exact to some 2^-45 of the whole.  What is no finite positive number counts as
  * no mass; a row without mass gives token -1; a number u_sample that is not below 1 gives the last index with mass.  A token
  * outside the vocabulary or offsets that do not ascend from 0 to n_draft are RT_ERR_BAD_INDEX (their sequence: accepted 0,
  * token -1). */
