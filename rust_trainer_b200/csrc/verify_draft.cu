@@ -1,6 +1,11 @@
 // Verification of drafted tokens: a cluster of CTAs a sequence.  Every CTA finds the first draft that does not stand (the draws are few);
 // then each warp sums a contiguous piece of the row that the next token is drawn from, the warps' sums go to all CTAs, and the warp whose
 // piece holds the token looks for it there, in the eighth of the piece that its own sums point to.  The row is read once.
+//
+// Measured: one sequence with four drafts over 151936 f32 13 to 15 us, 96 with up to eight over 128256 bf16 29 us (floor 5.7), 32 with up to three
+// certain ones over 151936 f32 21 to 24 us (3).  What bounds it: dependent loads (offsets, tokens, their probabilities, the row, the piece once
+// more), and for many sequences the arithmetic of exact sums, 57 % of all issue slots, in two waves of CTAs.  Clusters of four instead of eight took
+// 31 us for the 96 sequences and 23 for the one, 512 threads 42 for the 32; sums of two floats on packed pairs took more registers and the same time.
 #include "vocab_rows.cuh"
 
 namespace rt {

@@ -2,7 +2,7 @@
 
 Tolerances, with u = 2^-24 (half a step of f32, relative).  An exponential exp(x), x = (z - m) / T <= 0: the difference, the
 quotient and (where the kernel forms it) the product with log2 e are rounded, at most four times by u |x|, and the exponential
-itself is off by at most 4 u; a sum of such terms adds at most 64 roundings within a thread (what comes after is in 64 bits), and the
+itself is off by at most 4 u; a sum of such terms adds at most 64 roundings (within a thread, its warp, and of the warps), and the
 average of its terms' errors, at most 4 u times the mean |x| that the sum sees, which the factor 96 covers for |x| <= 8 where the mass is.
 So p is off by (4 |x| + 96) u p, a log-probability or log-sum-exp by 96 u + 4 u |x| and its own rounding u |s|.  What is written is
 rounded to its type: half a step, finfo.eps / 2 relative, or half of the smallest subnormal.  An exponential below 2^-126 is taken as 0
@@ -160,6 +160,18 @@ def test_top_logits_of_every_order(ctx, order, vocab):
         z = Rows(np.stack([ORDERS[order](vocab, rng) for _ in range(2)]), dtype)
         for k in (1, min(vocab, 33), min(vocab, 256)):
             _check_top(_top(ctx, z, k, 1.0), z, k, 1.0)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("vocab", [33, 300, 655, 1000, 2049])
+def test_top_logits_of_short_rows(ctx, vocab, dtype):
+    """Fewer vectors than threads, lists longer than there are vectors, more elements than are ranked by counting."""
+    rng = np.random.default_rng(vocab)
+    for offset in (0, 3):
+        z = Rows(_logits(rng, 5, vocab), dtype, vocab + offset, offset)
+        for k in {1, 29, 64, 65, 128, 129, 250, vocab}:
+            if k <= min(vocab, 256):
+                _check_top(_top(ctx, z, k, 1.0), z, k, 1.0)
 
 
 def test_top_logits_with_values_that_are_no_numbers(ctx):
@@ -508,6 +520,23 @@ def test_host_forms_are_the_device_forms(ctx):
     _check_verify(ops.verify_draft(ctx, p, q, tok, off, ua, us), P, Q, tok, off, ua, us)
     _check_verify(ops.verify_draft(ctx, p, None, tok, off, ua, us), P, None, tok, off, ua, us)
     assert ops.top_logits(ctx, v[:0], 3)[0].shape == (0, 3) and ops.softmax(ctx, v[:0]).shape == (0, 1003)
+
+
+@pytest.mark.parametrize("vocab", [640, 50021])
+def test_a_teacher_that_is_no_number_reaches_its_row_only(ctx, vocab):
+    """A NaN among a row's log-probabilities: with a renormalised list no entry's probability is known, with the rest as a bucket the rest's and
+    the entry's own are not."""
+    rng = np.random.default_rng(3)
+    z = Rows(_logits(rng, 3, vocab), "f32")
+    index = np.stack([rng.permutation(vocab)[:6] for _ in range(3)]).astype(np.int32)
+    t = np.log(np.full((3, 6), 0.1))
+    t[1, 2] = np.nan
+    for mode in ("tail", "renorm"):
+        loss, d = _distill(ctx, z, index, t, 1.0, mode, out="f32")[:2]
+        assert np.isfinite(loss[[0, 2]]).all() and np.isnan(loss[1])
+        unknown = np.isin(np.arange(vocab), index[1]) == (mode == "renorm")
+        unknown[index[1, 2]] = True
+        assert np.isfinite(d[[0, 2]]).all() and np.array_equal(np.isnan(d[1]), unknown)
 
 
 def test_refusals(ctx):

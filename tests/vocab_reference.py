@@ -55,7 +55,7 @@ def distill(z, index, t, temperature, mode, w=1.0):
         if mode == "tail":
             listed = np.zeros(n, bool)
             listed[v] = True
-            r = max(0.0, 1.0 - mass)
+            r = np.maximum(0.0, 1.0 - mass)  # a NaN stays
             zo = z[~listed]
             mo = zo.max() if zo.size else -np.inf
             if mo > -np.inf:
