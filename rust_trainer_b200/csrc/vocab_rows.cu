@@ -36,15 +36,16 @@ __device__ __forceinline__ void row_wait_turn(uint64_t* bars, uint32_t i, uint32
   row_wait(bars + (i & ((1u << turns_log2) - 1)), i >> turns_log2 & 1, status);
 }
 
-// The warps that sum.  The thread's reference is the largest of its first vectors: an exponential may be as large as 2^30 before it changes,
-// so that it rarely does.  KEEP (32-bit rows): the exponentials take their elements' place, for the warps that write.
+// The warps that sum.  A thread's reference is the largest of its warp's first vectors: an exponential may be as large as 2^10 before it changes,
+// so that it rarely does, and an exponent's rounding is small where the large ones are (with the thread's own, and up to 2^30, probabilities of f32
+// rows were off by 3 to 4e-7 instead of 1.4 to 2.5e-7).  KEEP (32-bit rows): the exponentials take their elements' place, for the warps that write.
 template <class T, int NT, bool KEEP>
 __device__ __forceinline__ void sum_rows(UnitRing<T, NT, ROW_STEP>& ring, const T* z, size_t ld, size_t rows, size_t row_step, const ExpT& ex, RowBars& b,
                                          float (*refs)[NT], RowStat (*stats)[VR_MAX_CLUSTER * (NT / 32)], uint32_t bytes, bool listed, bool give_back) {
   using Ring = UnitRing<T, NT, ROW_STEP>;
   constexpr int VEC = Ring::VEC, WARPS = NT / 32;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const float most = 30.0f / ex.hi;
+  const float most = 10.0f / ex.hi;
   uint32_t i = 0;
   for (size_t r = cluster_id(); r < rows; r += row_step, ++i) {
     ring.begin(z + r * ld);
@@ -69,7 +70,8 @@ __device__ __forceinline__ void sum_rows(UnitRing<T, NT, ROW_STEP>& ring, const 
         m = __hmax2_nan(m, __hmax2_nan(__hmax2_nan(*(const T2*)&v[1].x, *(const T2*)&v[1].y), __hmax2_nan(*(const T2*)&v[1].z, *(const T2*)&v[1].w)));
         top = max_nan(to_f32(m.x), to_f32(m.y));
       }
-      if (!(top <= ref + most) && ref == ref) {  // the first finite ones, ones that are far larger, a NaN, which stays
+      if (u == 0 || (!(top <= ref + most) && ref == ref)) {  // the first ones, ones that are far larger, a NaN, which stays
+        if (u == 0) top = warp_max_nan(top);
         if (ref > -INFINITY) {
           const float by = ex(ref - top);
 #pragma unroll
@@ -126,7 +128,7 @@ __device__ __forceinline__ void write_row(UnitRing<T, NT, ROW_STEP>& ring, O* ou
   constexpr int VEC = Ring::VEC;
   const bool aligned = ((uintptr_t)out - (uintptr_t)ring.align * sizeof(O)) % (VEC * sizeof(O) < 16 ? VEC * sizeof(O) : 16) == 0;
   const float ref = reference > -INFINITY ? reference : 0.0f;
-  // far below the reference in two factors: what is left of an exponential of 2^30 may be 2^30 larger than what one factor can say
+  // far below the reference in two factors: what is left of an exponential of 2^10 may be 2^10 larger than what one factor can say
   float h = 1.0f;
   if (sizeof(T) == 4 && mine > -INFINITY) {
     const bool far = (mine - reference) * ex.hi < -60.0f;
