@@ -56,7 +56,7 @@ __device__ __forceinline__ void sum_rows(UnitRing<T, NT, ROW_STEP>& ring, const 
     F2 acc[4] = {0, 0, 0, 0};
 #pragma unroll 1
     for (int u = 0; u < ring.n_units; ++u) {
-      ring.wait();
+      if (!listed) ring.wait();  // else the list's warps have waited
       uint4* const at = ring.unit() + tid;
       if (!listed && (u == 0 || u + 1 == ring.n_units)) ring.complete(u, at);
       const uint4 v[2] = {at[0], at[NT]};
@@ -139,8 +139,7 @@ __device__ __forceinline__ void write_row(UnitRing<T, NT, ROW_STEP>& ring, O* ou
   const F2 minus_ref = pack2(-ref, -ref), by = pack2(f, f), half_way = pack2(h, h);
 #pragma unroll 1
   for (int u = 0; u < ring.n_units; ++u) {
-    ring.wait();
-    const uint4* const at = ring.unit() + threadIdx.x % NT;
+    const uint4* const at = ring.unit() + threadIdx.x % NT;  // (the warps that sum have waited for it)
     const uint4 v[2] = {at[0], at[NT]};
     ring.release();
     ring.next();
