@@ -425,8 +425,8 @@ int launch_top_logits(rt_ctx* c, const VocabRows& z, size_t rows, int vocab, flo
     return with_threads(threads, [&](auto n) {
       using T = std::remove_pointer_t<decltype(zt)>;
       constexpr int NT = decltype(n)::value;
-      return launch_clusters(c, units == 1 ? top_logits_kernel<T, NT, true> : top_logits_kernel<T, NT, false>, true, rows, threads + 32, size, places * unit + other, (const T*)z.p, z.ld, rows, vocab,
-                             temperature, exp_t(temperature), k, index, logp, lse, places, room.kept, room.ranked, c->status_dev);
+      return launch_clusters(c, units == 1 ? top_logits_kernel<T, NT, true> : top_logits_kernel<T, NT, false>, true, rows, threads + 32, size,
+                             places * unit + other, (const T*)z.p, z.ld, rows, vocab, temperature, exp_t(temperature), k, index, logp, lse, places, room.kept, room.ranked, c->status_dev);
     });
   });
 }

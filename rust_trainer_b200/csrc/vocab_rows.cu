@@ -2,14 +2,14 @@
 // gone round.  In each CTA some warps sum row n + 1 while others write row n and the next ones are copied, so that memory is busy while sums
 // are found and go round, and a warp or a few make each row's list ready and find its loss.
 //
-// Measured, against the bytes at the rate of a copy: softmax of 1536 x 128256 bf16 into f32 203 us (floor 183, 5.8 TB/s); gradients of
-// 1024 x 151936 f32 in f16 from 64 entries 237 us (144), of 2048 x 128256 bf16 from 32 268 us (162); losses alone of 777 x 50021 f16
+// Measured, against the bytes at the rate of a copy: softmax of 1536 x 128256 bf16 into f32 207 us (floor 183, 5.7 TB/s); gradients of
+// 1024 x 151936 f32 in f16 from 64 entries 219 us (144), of 2048 x 128256 bf16 from 32 250 us (162); losses alone of 777 x 50021 f16
 // 37 us (12).  (All warps at one row after the other, with the same copies ahead: 285, 264, 283 and 37 us.)  What bounds distillation is the
-// chain of a row: its last unit's copy, the list, the sums (some 6500 cycles of the f32 row's 20000 over two rows), the exchange and the
-// coefficients (3000), the writing (6500), and two rows are all that a cluster's shared memory holds.  The warps that sum and those that write
-// share the issue slots, 46 % of which are taken over the whole.  Tried without gain: units in pairs (286 us: the warps that sum got faster,
-// those that write slower, and the code longer), lists that are taken out unit by unit so that sums begin behind the copy (267), two CTAs on an SM
-// with half of the row each (420 and more), the factor in the exponent for 16-bit results (the same).
+// chain of a row: its last unit's copy (some 4500 of the f32 row's 17300 cycles over two rows), the sums (4700), the exchange and the coefficients
+// (3200), the writing (4000), and two rows are all that a cluster's shared memory holds.  A wait on a barrier costs 100 to 200 cycles in
+// these loops: whoever is told of a whole row does not wait for its units (240 -> 219 us).  Tried without gain, in us for the f32 rows: units in pairs
+// (286), lists that are taken out unit by unit so that sums begin behind the copy (248), entries that each wait for their own unit (233), two CTAs
+// on an SM with half of the row each (420 and more), clusters that start one after the other, the factor in the exponent for 16-bit results (the same).
 //
 // What passes between the roles, row i of a CTA (all of them mbarriers, two or four in turn):
 //   full, empty   a unit has been copied; the warps that write the row (or, for a loss alone, that sum it) give it back
@@ -122,7 +122,9 @@ __device__ __forceinline__ void sum_rows(UnitRing<T, NT, ROW_STEP>& ring, const 
 
 // One row's results into `out`, by the warps that write: (16-bit rows) e f, e the exponentials relative to the row's reference, or (32-bit rows, whose
 // exponentials are there relative to the thread's reference `mine`) those times what that makes f.  Gives the units back.
-template <class O, class T, int NT>
+// PACED: with a wait for each unit, which the warps that sum have seen full already.  Where memory binds it spreads the stores: softmax of 1536 x
+// 128256 bf16 rows, one call after the other, takes 211 to 221 us with it and 229 without; distillation of 1024 x 151936 f32 rows 240 and 219.
+template <bool PACED, class O, class T, int NT>
 __device__ __forceinline__ void write_row(UnitRing<T, NT, ROW_STEP>& ring, O* out, float mine, float reference, float f, const ExpT& ex) {
   using Ring = UnitRing<T, NT, ROW_STEP>;
   constexpr int VEC = Ring::VEC;
@@ -139,7 +141,8 @@ __device__ __forceinline__ void write_row(UnitRing<T, NT, ROW_STEP>& ring, O* ou
   const F2 minus_ref = pack2(-ref, -ref), by = pack2(f, f), half_way = pack2(h, h);
 #pragma unroll 1
   for (int u = 0; u < ring.n_units; ++u) {
-    const uint4* const at = ring.unit() + threadIdx.x % NT;  // (the warps that sum have waited for it)
+    if (PACED) ring.wait();
+    const uint4* const at = ring.unit() + threadIdx.x % NT;
     const uint4 v[2] = {at[0], at[NT]};
     ring.release();
     ring.next();
@@ -219,7 +222,7 @@ softmax_rows_kernel(const T* z, size_t ld, size_t rows, int vocab, ExpT ex, O* p
       // a row of -inf has no probabilities, one with a NaN or +inf no number for them
       const float f = m == -INFINITY ? 0.0f : m < INFINITY ? 1.0f / sum : NAN;
       row_wait_turn(b.summed, i, 1, status);
-      write_row(ring, prob + r * prob_ld, refs[i & 1][tid - NT], m, f, ex);
+      write_row<true>(ring, prob + r * prob_ld, refs[i & 1][tid - NT], m, f, ex);
       __syncwarp();
       if ((tid & 31) == 0) mbar_arrive(b.done + (i & 1));
     }
@@ -326,7 +329,7 @@ distill_rows_kernel(const T* z, size_t ld, size_t rows, int vocab, float t, ExpT
       row_wait_turn(b.summed, i, 1, status);
       // (rows that nothing is learnt from, whatever their logits are, have zeros)
       if (!g.idle) {
-        write_row(ring, d + r * d_ld, refs[i & 1][tid - NT], g.reference, g.outside, ex);
+        write_row<false>(ring, d + r * d_ld, refs[i & 1][tid - NT], g.reference, g.outside, ex);
       } else {
         for (int u = 0; u < ring.n_units; ++u, ring.next()) {
           const float zero[VEC] = {};
@@ -507,15 +510,16 @@ distill_rows_kernel(const T* z, size_t ld, size_t rows, int vocab, float t, ExpT
   }
 }
 
-// How rows are held.  Threads that sum, and that write: few for short rows, of which an SM then holds several (registers admit five CTAs of 64
+// How rows are held.  Threads that sum, and that write: few for short rows, of which an SM then holds several (registers admit four CTAs of 64
 // threads, two of 128 or one of 256).  Distillation from 32 entries, by threads and the ring's KB:
 //   4096 rows of 640 f32   64 x 32: 33 us, 128 x 66: 49, 256 x 208: 94
 //   4096 of 2500 f32       64 x 32: 41, 128 x 66: 55, 256 x 208: 100
 //   4096 of 8000 f32       128 x 66: 68, 256 x 208: 102       2048 of them: 64 x 32: 49, 128 x 66: 41
 //   4096 of 16000 f32      128 x 66: 147, 256 x 208: 109
 // The CTAs of a row's cluster: as few as hold two rows, one that is summed and one that is written (longer rows have eight and are held once, at
-// least); 1024 rows of 151936 f32 took 238 us with six CTAs, 272 with eight and 330 with four, 2048 of 128256 bf16 268 with three, 287 with two
-// and 303 with four.  More where there are so few rows that SMs would be idle.  The ring's units: all that fit, as far as there are rows to fill them.
+// least); with some more waits than now 1024 rows of 151936 f32 took 246 us with six CTAs, 272 with eight and 330 with four, 2048 of 128256 bf16
+// 272 with three, 287 with two and 303 with four.  More where there are so few rows that SMs would be idle.  The ring's units: all that fit, as
+// far as there are rows to fill them.
 struct RowShape {
   int threads, cluster, places;
   size_t smem;

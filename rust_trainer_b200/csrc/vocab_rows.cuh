@@ -146,9 +146,6 @@ __device__ __forceinline__ void send(uint32_t to, uint32_t bar, uint32_t a, uint
   asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(to), "r"(a), "r"(b), "r"(c), "r"(d), "r"(bar)
                : "memory");
 }
-__device__ __forceinline__ void send(uint32_t to, uint32_t bar, double v) {
-  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.b64 [%0], %1, [%2];" ::"r"(to), "l"(__double_as_longlong(v)), "r"(bar) : "memory");
-}
 // barriers of some of a CTA's warps
 template <int NT>
 __device__ __forceinline__ void work_sync() { asm volatile("bar.sync 1, %0;" ::"n"(NT) : "memory"); }
