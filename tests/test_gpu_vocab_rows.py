@@ -522,6 +522,50 @@ def test_host_forms_are_the_device_forms(ctx):
     assert ops.top_logits(ctx, v[:0], 3)[0].shape == (0, 3) and ops.softmax(ctx, v[:0]).shape == (0, 1003)
 
 
+class Picked:
+    """Some rows of a call, for the checks."""
+
+    def __init__(self, z, at):
+        self.f64, self.rows, self.vocab, self.dtype = z.f64[at], len(at), z.vocab, z.dtype
+
+
+@pytest.mark.parametrize("rows,vocab,dtype", [(2600, 640, "f32"), (2600, 1003, "bf16"), (1500, 7000, "f32"), (1300, 9001, "f16"), (450, 50021, "f32"),
+                                              (700, 50021, "bf16"), (130, 151936, "f32")])
+def test_many_rows_follow_one_another(ctx, rows, vocab, dtype):
+    """Several rows for each cluster, of which none may find what another one left: steep, even, masked and far-off ones, ones that are no numbers and ones of
+    no weight, in turn."""
+    rng = np.random.default_rng(rows + vocab)
+    v = _logits(rng, rows, vocab)
+    v[1::7] *= 30
+    v[2::7] = 1.5
+    v[3::7, vocab // 3:] = -np.inf
+    v[4::7] += 4096
+    v[5::21, vocab // 2] = np.nan
+    v[6::21] = -np.inf
+    z = Rows(v, dtype, vocab + 3, 1)
+    k = 40
+    index = rng.integers(0, vocab, (rows, k)).astype(np.int32)
+    index[::5, 30:] = -1
+    t = np.log(rng.dirichlet(np.ones(k), rows) * rng.uniform(0.3, 1.0, (rows, 1)))
+    weight = rng.uniform(0.2, 1.5, rows)
+    weight[::9] = 0
+    at = np.unique(np.concatenate([np.arange(0, rows, max(1, rows * vocab // 1500000)), np.arange(rows - 30, rows)]))
+    some = Picked(z, at)
+    for mode in ("tail", "renorm"):
+        for out in (dtype, None):
+            ls, d, f, _ = _distill(ctx, z, index, t, 1.0, mode, weight, out)
+            _check_distill((ls[at], None if d is None else d[at], f[at], None), some, index[at], t[at], 1.0, mode, weight[at], out)
+    p = Rows(np.full((rows, vocab), np.nan), "f32")
+    _before()
+    ctx.check(rt.lib().rt_softmax_dev(ctx._h, z.ptr, DT[dtype], rows, vocab, z.ld, 1.0, p.ptr, 0, p.ld))
+    _sync(ctx)
+    _check_prob(p.read()[at], some, 1.0, "f32")
+    at = at[~np.isnan(some.f64).any(1)]  # (their order takes long to find in 64 bits)
+    for top in (9, 100):
+        _check_top([x[at] for x in _top(ctx, z, top, 1.0)], Picked(z, at), top, 1.0)
+    assert z.others_untouched()
+
+
 @pytest.mark.parametrize("vocab", [640, 50021])
 def test_a_teacher_that_is_no_number_reaches_its_row_only(ctx, vocab):
     """A NaN among a row's log-probabilities: with a renormalised list no entry's probability is known, with the rest as a bucket the rest's and
