@@ -2,10 +2,10 @@
 // then each warp sums a contiguous piece of the row that the next token is drawn from, the warps' sums go to all CTAs, and the warp whose
 // piece holds the token looks for it there, in the eighth of the piece that its own sums point to.  The row is read once.
 //
-// Measured: one sequence with four drafts over 151936 f32 13 to 15 us, 96 with up to eight over 128256 bf16 29 us (floor 5.7), 32 with up to three
+// Measured: one sequence with four drafts over 151936 f32 12 to 15 us, 96 with up to eight over 128256 bf16 25 us (floor 5.7), 32 with up to three
 // certain ones over 151936 f32 21 to 24 us (3).  What bounds it: dependent loads (offsets, tokens, their probabilities, the row, the piece once
-// more), and for many sequences the arithmetic of exact sums, 57 % of all issue slots, in two waves of CTAs.  Clusters of four instead of eight took
-// 31 us for the 96 sequences and 23 for the one, 512 threads 42 for the 32; sums of two floats on packed pairs took more registers and the same time.
+// more), and for many sequences the arithmetic of exact sums, 57 % of all issue slots.  512 threads took 42 us for the 32; sums of two floats on packed
+// pairs took more registers and the same time.
 #include "vocab_rows.cuh"
 
 namespace rt {
@@ -228,7 +228,12 @@ __global__ void __launch_bounds__(VD_THREADS) verify_draft_kernel(const T* P, si
 }
 
 int launch_verify_draft(rt_ctx* c, const VerifyArgs& a) {
-  const int size = a.vocab >= 8192 ? 8 : a.vocab >= 2048 ? 2 : 1;
+  // As many CTAs a sequence as run at once for all of them, three on an SM: a second wave costs more than a longer row.  In us, by the cluster's size:
+  //   1 of 30000 f32   1: 20.2, 2: 14.3, 4 and 8: 12.3       1 of 6000 f32: the same with any
+  //   64 of 30000 f32   1: 32.8, 2: 22.5, 4: 17.7, 8: 24.0    96 of 128256 bf16   2: 41.0, 4: 30.7, 8: 34.6
+  //   200 of 128256 bf16   1: 74, 2: 52, 4: 53, 8: 58         1000 of 9000 bf16   1: 39, 2: 61, 8: 202
+  int size = 1;
+  while (a.vocab >= 8192 && size < VR_MAX_CLUSTER && (size_t)a.n_seq * size * 2 <= 3 * (size_t)c->num_sms) size *= 2;
   return with_dtype(a.p.dtype, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
     return launch_clusters(c, verify_draft_kernel<T>, false, a.n_seq, VD_THREADS, size, 0, (const T*)a.p.p, a.p.ld, (const T*)a.q.p, a.q.ld, a.vocab, a.tok, a.offsets,
