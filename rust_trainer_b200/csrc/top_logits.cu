@@ -14,13 +14,14 @@
 
 namespace rt {
 
-// Elements that are kept on the way, and that are ranked, at most: in proportion to what random rows need, some 12 k and 2 k.
+// Elements that are kept on the way, and that are ranked, at most: in proportion to what random rows need, some 12 k and 2 k (in a cluster, where each
+// CTA may hold k by its own bound, 2 k each: with 256 each, 200 of 30 rows of 151936 f32 took 125 us for want of room, and 36 with one CTA a row).
 struct TopRoom {
   int kept, ranked;
 };
 constexpr int TOP_SHORT = 128;  // entries of a list that 256 threads make: 128 of 1475 x 20000 f32 took 80 us with them, 119 with 512
 static TopRoom top_room(int k, int cluster) {
-  return {k <= 64 ? 1536 : k <= TOP_SHORT ? 2048 : 3584, cluster > 1 ? 256 * cluster : k <= TOP_SHORT ? 768 : 1024};
+  return {k <= 64 ? 1536 : k <= TOP_SHORT ? 2048 : 3584, cluster > 1 ? (k <= 64 ? 256 : k <= TOP_SHORT ? 384 : 640) * cluster : k <= TOP_SHORT ? 768 : 1024};
 }
 static_assert(RT_TOP_MAX <= 256, "k elements of one CTA's share have to fit");
 // An element as an integer, all different: its value's order above, the lower index in front.
@@ -413,14 +414,16 @@ top_logits_kernel(const T* z, size_t ld, size_t rows, int vocab, float t, ExpT e
 }
 
 int launch_top_logits(rt_ctx* c, const VocabRows& z, size_t rows, int vocab, float temperature, int k, int* index, float* logp, float* lse) {
-  // Long lists want more threads, whose maxima are the sample that the bound is found in.  Three CTAs on an SM, or one; more CTAs a row
-  // where there are few rows.
+  // Long lists want more threads, whose maxima are the sample that the bound is found in.  Three CTAs on an SM, or one; more CTAs a row where there are
+  // few rows, as long as two find room on an SM: 32 of 64 rows of 151936 f32 took 36 us with one, 27 with two, 25 with four and 37 with eight; of
+  // 128 rows 39, 33, 41 and 57.
   const int threads = k <= TOP_SHORT ? 256 : 512, vec = z.dtype == RT_DT_F32 ? 4 : 8, units = (vec - 1 + vocab + 16 * threads - 1) / (16 * threads);
   int size = 1;
-  while (size * 2 <= VR_MAX_CLUSTER && units > size && rows * size * 2 <= (size_t)c->num_sms) size *= 2;
+  const size_t at_once = (threads == 256 ? 2 : 1) * (size_t)c->num_sms;
+  while (size * 2 <= VR_MAX_CLUSTER && units > size && rows * size * 2 <= at_once) size *= 2;
   const TopRoom room = top_room(k, size);
   const size_t other = (room.kept + room.ranked) * sizeof(TopKey), unit = (size_t)threads * 16 * (z.dtype == RT_DT_F32 ? 4 : 2);
-  const int places = (int)std::min(((threads == 256 ? 70 : 208) * 1024 - other) / unit, (size_t)VR_MAX_UNITS);
+  const int places = (int)std::min(((threads != 256 ? 208 : size > 1 ? 104 : 70) * 1024 - other) / unit, (size_t)VR_MAX_UNITS);
   return with_dtype(z.dtype, [&](auto* zt) {
     return with_threads(threads, [&](auto n) {
       using T = std::remove_pointer_t<decltype(zt)>;
