@@ -99,6 +99,7 @@ top_logits_kernel(const T* z, size_t ld, size_t rows, int vocab, float t, ExpT e
   __shared__ uint64_t bars[2 * VR_MAX_UNITS + 2];
   __shared__ TopStat stats[2][VR_MAX_CLUSTER * WARPS];
   __shared__ uint2 told[2][VR_MAX_CLUSTER];  // what every CTA told
+  __shared__ uint2 met[VR_MAX_CLUSTER];  // never read: that something came is all it says
   __shared__ uint32_t sample[32 * SAMPLE_LANE];
   __shared__ double s_lse, s_sums[WARPS];
   __shared__ int s_kept, s_n, s_count[2], s_found[VR_MAX_CLUSTER];
@@ -362,7 +363,10 @@ top_logits_kernel(const T* z, size_t ld, size_t rows, int vocab, float t, ExpT e
       for (int i = 0; i < ring.size; ++i) n += (int)found[i].x;
       if (tid < ring.size) s_found[tid] = (int)found[tid].x;  // what was told may be overwritten once this exchange is over
       work_sync<NT>();
-      if (tid == 0) exchange.expect((uint32_t)(n - n_mine) * 8);
+      // A word from everybody comes with them, behind the barrier: nobody goes on to the next row, and tells of it, where `found` is still read.  A
+      // CTA that has all elements of the row would wait for no others.
+      if (tid == 0) exchange.expect((uint32_t)(n - n_mine + ring.size) * 8);
+      if (tid < ring.size) send(mapa_u32(smem_u32(met + ring.rank), tid), exchange.bar(tid), 0u, 0u);
       for (int i = tid; i < n_mine; i += NT) {
         const uint2 key = *(const uint2*)(mine + i);
         for (int o = 0; o < ring.size; ++o)

@@ -1,0 +1,28 @@
+"""The row operations over the vocabulary where their numbers or their arguments are at an end of what is allowed, and rows of a call that
+holds a bad one.  Tolerances: those of test_gpu_vocab_rows.py, whose derivation covers every case here."""
+import numpy as np
+import pytest
+
+import rust_trainer_b200 as rt
+import vocab_reference as R
+from rust_trainer_b200 import ops
+from test_gpu_vocab_rows import DT, U, Rows, _before, _check_distill, _check_prob, _check_top, _check_verify, _dev, _distill, _drafts, _empty, _lists, _logits, _sync, _top, _verify
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("k", [1, 5, 130])
+def test_clusters_that_take_several_rows_and_find_all_in_one_place(ctx, k):
+    """The largest elements of a row lie in one CTA's units, so that it waits for nobody's; the cluster goes on to the next row."""
+    rng = np.random.default_rng(k)
+    for rows, vocab in ((37, 50021), (19, 100003), (74, 20011), (146, 9001)):
+        v = _logits(rng, rows, vocab)
+        for r in range(rows):
+            at = rng.integers(0, vocab - k)
+            v[r, at:at + k] += 100.0
+        z = Rows(v, "f32")
+        want = _top(ctx, z, k, 1.0)
+        _check_top(want, z, k, 1.0)
+        for _ in range(10):
+            got = _top(ctx, z, k, 1.0)
+            assert all(np.array_equal(a, b) for a, b in zip(got, want))
