@@ -15,6 +15,7 @@
 //   full, empty   a unit has been copied; the warps that write the row (or, for a loss alone, that sum it) give it back
 //   patched       the list's warps have taken the listed elements out of the row
 //   summed        the row's exponentials and references are there
+//   listed        the list's entries are there, for the warp that writes their gradients (what is sent to `exchange` says nothing of them)
 //   exchange      all CTAs' sums of the row, and what their lists say, have come
 //   written       by the warps that write
 //   done          the row has been written, its listed elements too, and its loss found; row i + 2 may take its references' and its list's places.
@@ -26,7 +27,7 @@ namespace rt {
 
 constexpr int ROW_STEP = 2;  // vectors of a thread in a unit
 struct RowBars {
-  uint64_t units[2 * VR_MAX_UNITS], exchange[4], summed[2], written[2], done[2], patched[2];
+  uint64_t units[2 * VR_MAX_UNITS], exchange[4], summed[2], written[2], done[2], patched[2], listed[2];
 };
 // What a warp knows of its share of a row, and sends to every CTA of the cluster: a reference, and the sum of exponentials relative to it.
 struct alignas(8) RowStat {
@@ -310,6 +311,7 @@ distill_rows_kernel(const T* z, size_t ld, size_t rows, int vocab, float t, ExpT
     mbar_init(b.written + tid, WARPS);
     mbar_init(b.done + tid, 1);
     mbar_init(b.patched + tid, list_warps);
+    mbar_init(b.listed + tid, list_warps);
   }
   mbar_fence_init();
   cluster_sync_all();  // nobody sends to a CTA that does not run yet
@@ -373,6 +375,7 @@ distill_rows_kernel(const T* z, size_t ld, size_t rows, int vocab, float t, ExpT
       }
       if (d) {
         const RowGradient g = row_gradient<WARPS>(stat, list, ring.size, w == 0.0f, row_scale ? 1.0f : w / t, ex);
+        row_wait_turn(b.listed, i, 1, status);
         row_wait_turn(b.written, i, 1, status);
         for (int j = lane; j < k; j += 32) {
           const int c = s_mine[i & 1][j];
@@ -480,6 +483,8 @@ distill_rows_kernel(const T* z, size_t ld, size_t rows, int vocab, float t, ExpT
         s_q[i & 1][me] = q_all;
       }
       s_mine[i & 1][me] = first ? my : -1;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(b.listed + (i & 1));
       double mass = q, cross = q > 0.0 ? q * (lt - x_my) : q, on = first ? e : 0.0;
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) {

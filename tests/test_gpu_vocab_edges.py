@@ -26,3 +26,20 @@ def test_clusters_that_take_several_rows_and_find_all_in_one_place(ctx, k):
         for _ in range(10):
             got = _top(ctx, z, k, 1.0)
             assert all(np.array_equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("rows,vocab", [(1200, 640), (500, 9001), (40, 50021)])
+def test_every_row_has_the_gradients_of_its_own_list(ctx, rows, vocab):
+    """Long lists with indices that come twice, another one for each of many rows that follow one another: all listed gradients of all rows."""
+    rng = np.random.default_rng(rows)
+    k = 256
+    z = Rows(_logits(rng, rows, vocab), "f32")
+    index = rng.integers(0, vocab, (rows, k)).astype(np.int32)
+    index[::2] = np.argsort(rng.random((rows, vocab)), axis=1)[::2, :k]  # every second list without repetition
+    t = np.log(rng.dirichlet(np.ones(k), rows) * rng.uniform(0.3, 1.0, (rows, 1)))
+    for mode in ("tail", "renorm"):
+        got = _distill(ctx, z, index, t, 1.0, mode, None, "f32")
+        _check_distill(got, z, index, t, 1.0, mode, None, "f32")
+        for _ in range(5):
+            again = _distill(ctx, z, index, t, 1.0, mode, None, "f32")
+            assert np.array_equal(again[0], got[0]) and np.array_equal(again[1], got[1])
