@@ -259,6 +259,7 @@ top_logits_kernel(const T* z, size_t ld, size_t rows, int vocab, float t, ExpT e
     TopStat* stat = stats[exchange.turn()];
     uint2* to = told[exchange.turn()];
     const int n_kept = s_kept;  // all have been counted before the bound's barriers
+    // (What was told may be anything once a wait has run out: no count is taken for more than there is room, and no loop goes by them alone.)
     if (tid == 0) exchange.expect(warps * sizeof(TopStat) + ring.size * 8);
     if (lane < ring.size)
       send(mapa_u32(smem_u32(&stat[ring.rank * WARPS + warp]), lane), exchange.bar(lane), __float_as_uint(st.R), __float_as_uint(st.s), __float_as_uint(st.m), 0u);
@@ -289,7 +290,7 @@ top_logits_kernel(const T* z, size_t ld, size_t rows, int vocab, float t, ExpT e
       if (p < room_each) mine[p] = key;
     };
     if (fits) {
-      for (int i = tid; i < n_kept; i += NT)
+      for (int i = tid; i < min(n_kept, kept_most); i += NT)
         if (kept[i] >= (TopKey)bound << TOP_INDEX_BITS) push(kept[i]);
     }
     work_sync<NT>();
@@ -342,8 +343,8 @@ top_logits_kernel(const T* z, size_t ld, size_t rows, int vocab, float t, ExpT e
       // low is reached by k elements, high by fewer; elements are all different, so that some key between is reached by exactly k
       TopKey low = (TopKey)bound << TOP_INDEX_BITS, high = (TopKey)1 << (32 + TOP_INDEX_BITS);
       bool room_for_all = false;
-      // the first question: are the bound's ties the matter?
-      for (TopKey mid = min(low + ((TopKey)1 << TOP_INDEX_BITS), high - 1); !room_for_all; mid = low + (high - low) / 2) {
+      // the first question: are the bound's ties the matter?  (Then at most one for each bit of a key.)
+      for (TopKey mid = min(low + ((TopKey)1 << TOP_INDEX_BITS), high - 1); !room_for_all && round < 64; mid = low + (high - low) / 2) {
         const int n = count(mid, &room_for_all);
         room_for_all &= n >= k;
         if (n >= k) low = mid;
@@ -357,11 +358,12 @@ top_logits_kernel(const T* z, size_t ld, size_t rows, int vocab, float t, ExpT e
       work_sync<NT>();
       found = tell((uint32_t)s_n, 0);
     }
-    int n_mine = (int)found[ring.rank].x;
+    auto n_found = [&](int i) { return (int)min(found[i].x, (uint32_t)room_each); };
+    int n_mine = n_found(ring.rank);
     if (ring.size > 1) {  // everybody's to everybody
       int n = 0;
-      for (int i = 0; i < ring.size; ++i) n += (int)found[i].x;
-      if (tid < ring.size) s_found[tid] = (int)found[tid].x;  // what was told may be overwritten once this exchange is over
+      for (int i = 0; i < ring.size; ++i) n += n_found(i);
+      if (tid < ring.size) s_found[tid] = n_found(tid);  // what was told may be overwritten once this exchange is over
       work_sync<NT>();
       // A word from everybody comes with them, behind the barrier: nobody goes on to the next row, and tells of it, where `found` is still read.  A
       // CTA that has all elements of the row would wait for no others.
