@@ -56,7 +56,8 @@ __device__ __forceinline__ uint32_t warp_sort(uint32_t v) {
 // together, and sums with different R meet exactly.  What hi leaves out is another temperature by 2^-26 or so: the row's log-sum-exp makes up for it,
 // as far as the mass is near the row's maximum.  R is set by the first elements, and again when one is 2^60 times as large, so rarely.
 // Elements that are too large or too far down for such an R (beyond 2^22 in units of T / log2(e)) have none: R = inf, or stays -inf, and a
-// row that has no other is summed again, relative to its maximum.
+// row where that matters, one whose own R is inf or not well above the least one, is summed again, relative to its maximum.
+constexpr float TOP_MOST_R = 4194304.0f;
 struct RunningSum {
   float R = -INFINITY, most = -INFINITY;  // most: elements up to here need no other R
   F2 s[2] = {0, 0};
@@ -64,11 +65,11 @@ struct RunningSum {
     if (!(largest <= most)) {
       if (R == R) {  // a NaN stays
         const float to = largest == largest ? ceilf(largest * hi) : NAN;
-        if (!(to < -4194304.0f)) {
+        if (!(to < -TOP_MOST_R)) {
           const float by = R > -INFINITY ? ex2(R - to) : 0.0f;
           s[0] = mul2(s[0], pack2(by, by));
           s[1] = mul2(s[1], pack2(by, by));
-          R = to > 4194304.0f ? INFINITY : to;
+          R = to > TOP_MOST_R ? INFINITY : to;
           most = (R + 60.0f) / hi;
         }
       }
@@ -269,7 +270,8 @@ top_logits_kernel(const T* z, size_t ld, size_t rows, int vocab, float t, ExpT e
     for (int i = lane; i < warps; i += 32) m = max_nan(m, stat[i].m), R = max_nan(R, stat[i].R);
     m = warp_max_nan(m);
     R = warp_max_nan(R);
-    const bool bad = !(m < INFINITY), again = !bad && m > -INFINITY && !(R > -INFINITY && R < INFINITY);
+    // (R 64 above the least one: an element that was left out is at most 2^-64 of the row's sum)
+    const bool bad = !(m < INFINITY), again = !bad && m > -INFINITY && !(R >= 64.0f - TOP_MOST_R && R < INFINITY);
     if (warp == WARPS - 1 && !again) {
       double all = 0.0;
       for (int i = lane; i < warps; i += 32)

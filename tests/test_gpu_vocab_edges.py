@@ -43,3 +43,19 @@ def test_every_row_has_the_gradients_of_its_own_list(ctx, rows, vocab):
         for _ in range(5):
             again = _distill(ctx, z, index, t, 1.0, mode, None, "f32")
             assert np.array_equal(again[0], got[0]) and np.array_equal(again[1], got[1])
+
+
+@pytest.mark.parametrize("k", [2, 200])
+@pytest.mark.parametrize("rows,vocab", [(23, 50021), (23, 1003), (400, 9000)])
+@pytest.mark.parametrize("temperature", [1.0, 0.01, 1e-4, 1e4])
+def test_top_logits_about_the_largest_exponents(ctx, temperature, rows, vocab, k):
+    """z log2(e) / T about -2^22 and 2^22, on both sides of the border in one row: every element has its share of the sum."""
+    rng = np.random.default_rng(rows)
+    border = 2.0**22 * np.log(2.0) * temperature
+    v = np.empty((rows, vocab))
+    for r in range(rows):
+        sign = -1.0 if r % 4 else 1.0
+        v[r] = sign * border + temperature * (0.25 * (r % 23 - 11) + (rng.uniform(-2, 2, vocab) if r % 2 else 0.0))
+        v[r, rng.integers(0, vocab)] += 0.5 * temperature
+    z = Rows(v, "f32")
+    _check_top(_top(ctx, z, k, temperature), z, k, temperature)
