@@ -238,7 +238,8 @@ rt_status rt_top_logits_dev(rt_ctx* ctx, const void* logits_dev, int dtype, size
  * and the teacher's log-probability t_j at it, as rt_top_logits_dev writes them.  An index that comes twice counts twice:
  * the probabilities add up.
  *   RENORM: q_j = exp(t_j) / sum exp(t);  loss = w sum q_j (log q_j - s_{i_j});  dz_v = (w / T) (p_v - q_v);
- *           a row whose list has no mass gets 0 for both
+ *           the t_j count up to a constant, since exponentials and their sum are held in 64 bits (t_j up to 690); a row whose
+ *           list has no mass (less than 1e-300) gets 0 for both
  *   TAIL:   q_j = exp(t_j), r = max(0, 1 - sum q), R = the student's mass outside the list;
  *           loss = w (sum q_j (t_j - s_{i_j}) + r (log r - log R));
  *           dz_v = (w / T) (p_v - q_v) inside the list, (w / T) p_v (1 - r / R) outside

@@ -235,11 +235,11 @@ softmax_rows_kernel(const T* z, size_t ld, size_t rows, int vocab, ExpT ex, O* p
 // What a CTA's list says of a row: the sum of its listed elements' exponentials, relative to the largest logit listed; what the teacher has
 // left (-1: the list has no mass that the student could learn from); by what its probabilities are divided, inverted; the largest logit.
 struct alignas(16) ListStat {
-  double listed;
-  float rest, by;
-  float top, listed32, unused[2];
-  static constexpr int SENT = 24;
+  double listed, by;  // (64 bits: what host lists call log-probabilities may be far from 0, all of them)
+  float rest, top, listed32, unused;
 };
+// a list of less mass than this has none
+constexpr double LEAST_MASS = 1e-300;
 // what a list leaves of a teacher's mass; a NaN stays
 __device__ __forceinline__ double left_of(double mass) { return mass > 1.0 ? 0.0 : 1.0 - mass; }
 struct alignas(16) LossStat {  // the teacher's mass, and sum q (t_j - z_j / T), the z relative to the largest
@@ -248,7 +248,8 @@ struct alignas(16) LossStat {  // the teacher's mass, and sum q (t_j - z_j / T),
 // What a row's sums make of it: a gradient outside of the list is exp(z - reference) outside, one on it e listed - q by, e relative to the largest
 // listed.  (Few instructions: run once a row between loops that do not leave them in the caches, each line of them is waited for.)
 struct RowGradient {
-  float reference, outside, listed, by;
+  float reference, outside, listed;
+  double by;
   bool idle;
 };
 template <int WARPS>
@@ -318,7 +319,7 @@ distill_rows_kernel(const T* z, size_t ld, size_t rows, int vocab, float t, ExpT
   const size_t row_step = gridDim.x / (unsigned)ring.size;
   const int writers = d ? NT : 0, copier = NT + writers, finisher = copier + 32, lister = finisher + 32;
   if (tid < NT) {
-    const uint32_t bytes = ring.size * WARPS * sizeof(RowStat) + ring.size * ListStat::SENT + (finds_loss ? sizeof(LossStat) : 0);
+    const uint32_t bytes = ring.size * WARPS * sizeof(RowStat) + ring.size * sizeof(ListStat) + (finds_loss ? sizeof(LossStat) : 0);
     if (d) sum_rows<T, NT, sizeof(T) == 4>(ring, z, ld, rows, row_step, ex, b, refs, stats, bytes, true, false);
     else sum_rows<T, NT, false>(ring, z, ld, rows, row_step, ex, b, refs, stats, bytes, true, true);
   } else if (tid < copier) {  // writes
@@ -370,7 +371,7 @@ distill_rows_kernel(const T* z, size_t ld, size_t rows, int vocab, float t, ExpT
           double l = mass == 0.0 ? 0.0 : top > -INFINITY ? cross + mass * (log_sum + (above ? x : 0.0)) : INFINITY;
           if (!tail) l = l / mass - log_mass;
           if (rest > 0.0) l += so > 0.0 ? rest * (log_rest - log_so + log_sum - (above ? 0.0 : x)) : INFINITY;
-          loss[r] = w == 0.0f || (!tail && mass == 0.0) ? 0.0f : !(max_nan(mo, top) < INFINITY) ? NAN : (float)(w * l);
+          loss[r] = w == 0.0f || (!tail && mass < LEAST_MASS) ? 0.0f : !(max_nan(mo, top) < INFINITY) ? NAN : (float)(w * l);
         }
       }
       if (d) {
@@ -497,12 +498,13 @@ distill_rows_kernel(const T* z, size_t ld, size_t rows, int vocab, float t, ExpT
       if (warp == 0) {
         mass = cross = on = 0.0;
         for (int j = 0; j < list_warps; ++j) mass += s_sums[j][0], cross += s_sums[j][1], on += s_sums[j][2];
-        const float rest = tail ? (float)left_of(mass) : mass == 0.0 ? -1.0f : 0.0f, by = tail ? 1.0f : 1.0f / (float)mass;
+        const float rest = tail ? (float)left_of(mass) : mass < LEAST_MASS ? -1.0f : 0.0f;
+        const double by = tail ? 1.0 : 1.0 / mass;
         const uint64_t* bar = b.exchange + (i & 3);
         if (lane < ring.size) {
           const uint32_t to = mapa_u32(smem_u32(&lists[i & 3][ring.rank]), lane), its_bar = mapa_u32(smem_u32(bar), lane);
-          send(to, its_bar, (uint32_t)__double2loint(on), (uint32_t)__double2hiint(on), __float_as_uint(rest), __float_as_uint(by));
-          send(to + 16, its_bar, __float_as_uint(top), __float_as_uint((float)on));
+          send(to, its_bar, (uint32_t)__double2loint(on), (uint32_t)__double2hiint(on), (uint32_t)__double2loint(by), (uint32_t)__double2hiint(by));
+          send(to + 16, its_bar, __float_as_uint(rest), __float_as_uint(top), __float_as_uint((float)on), 0u);
         }
         if (finds_loss && lane == 0)
           send(mapa_u32(smem_u32(&losses[i & 3]), 0), mapa_u32(smem_u32(bar), 0), (uint32_t)__double2loint(mass), (uint32_t)__double2hiint(mass),

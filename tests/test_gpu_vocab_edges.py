@@ -59,3 +59,26 @@ def test_top_logits_about_the_largest_exponents(ctx, temperature, rows, vocab, k
         v[r, rng.integers(0, vocab)] += 0.5 * temperature
     z = Rows(v, "f32")
     _check_top(_top(ctx, z, k, temperature), z, k, temperature)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("shift", [-100, -600, 90, 600, -2000])
+def test_renormalised_lists_of_any_magnitude(ctx, shift, dtype):
+    """log-probabilities up to a constant are the same list, however small or large their exponentials are; a mass below 1e-300 is none."""
+    rng = np.random.default_rng(5)
+    vocab, k = 3001, 40
+    z = Rows(_logits(rng, 6, vocab), dtype)
+    index, t = _lists(rng, z, k, 1.0)
+    t = np.round(t * 256) / 256  # so that the constant is added exactly
+    index[1, 7:] = -1
+    index[2, 1::2] = index[2, 0]
+    t[3, 5:] = -np.inf
+    index[4] = -1
+    t[5] = -np.inf
+    weight = rng.uniform(0.2, 1.5, 6)
+    for out, factor in (("f32", False), ("f16", True)):
+        got = _distill(ctx, z, index, t + shift, 1.3, "renorm", weight, out, factor=factor)
+        if shift > -700:
+            _check_distill(got, z, index, t, 1.3, "renorm", weight, out, factor=factor)
+        empty = slice(4 if shift > -700 else 0, 6)
+        assert (got[0][empty] == 0).all() and (got[1][empty] == 0).all()
