@@ -74,16 +74,17 @@ __device__ __forceinline__ void sum_rows(UnitRing<T, NT, ROW_STEP>& ring, const 
       if (u == 0 || (!(top <= ref + most) && ref == ref)) {  // the first ones, ones that are far larger, a NaN, which stays
         if (u == 0) top = warp_max_nan(top);
         if (ref > -INFINITY) {
-          const float by = ex(ref - top);
+          const bool far = KEEP && (ref - top) * ex.hi < -60.0f;  // in two factors, as in write_row
+          const float by = ex(far ? 0.5f * (ref - top) : ref - top), then = far ? by : 1.0f;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) acc[j] = mul2(acc[j], pack2(by, by));
+          for (int j = 0; j < 4; ++j) acc[j] = mul2(mul2(acc[j], pack2(by, by)), pack2(then, then));
           if constexpr (KEEP) {
 #pragma unroll 1
             for (int k = 0, place = first_place; k < u; ++k) {
 #pragma unroll
               for (int j = 0; j < ROW_STEP; ++j) {
                 float4* e = (float4*)(ring.slots + place * Ring::UNIT + j * NT + tid);
-                *e = make_float4(e->x * by, e->y * by, e->z * by, e->w * by);
+                *e = make_float4(e->x * by * then, e->y * by * then, e->z * by * then, e->w * by * then);
               }
               if (++place == ring.places) place = 0;
             }

@@ -82,3 +82,22 @@ def test_renormalised_lists_of_any_magnitude(ctx, shift, dtype):
             _check_distill(got, z, index, t, 1.3, "renorm", weight, out, factor=factor)
         empty = slice(4 if shift > -700 else 0, 6)
         assert (got[0][empty] == 0).all() and (got[1][empty] == 0).all()
+
+
+def _steps(vocab):
+    """A row that rises late: zeros in the first vectors of every CTA, then values some 2^10 times as likely, then one that leaves those at 2^-117."""
+    v = np.zeros(vocab, np.float32)
+    v[vocab // 2:] = 6.9
+    v[-3] = 88.0
+    return v
+
+
+@pytest.mark.parametrize("rows,vocab", [(160, 2100), (160, 12000), (2, 65536)])
+def test_softmax_of_rows_that_rise_late(ctx, rows, vocab):
+    """Probabilities down to 2^-126 of the largest are there, wherever the largest lies."""
+    z = Rows(np.tile(_steps(vocab), (rows, 1)), "f32")
+    p = Rows(np.full((rows, vocab), np.nan), "f32")
+    _before()
+    ctx.check(rt.lib().rt_softmax_dev(ctx._h, z.ptr, 0, rows, vocab, vocab, 1.0, p.ptr, 0, vocab))
+    _sync(ctx)
+    _check_prob(p.read(), z, 1.0, "f32")
