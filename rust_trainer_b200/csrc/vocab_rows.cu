@@ -260,7 +260,10 @@ __device__ __forceinline__ RowGradient row_gradient(const RowStat* stat, const L
   const int lane = threadIdx.x & 31;
   const float2 sums = warp_sum_f32x2(join_stats<WARPS>(stat, size, ex, &mo), lane < size ? list[lane].listed32 : 0.0f);
   const float so = sums.x, on = sums.y, top = list[0].top, rest = list[0].rest, m = max_nan(mo, top);
-  const float rest_to = mo > -INFINITY ? ex(mo - m) : 0.0f, top_to = top > -INFINITY ? ex(top - m) : 0.0f;
+  // (exponentials outside may be 2^10 times their reference's, so that what makes them the row's is said down to subnormal numbers)
+  const bool far = (mo - m) * ex.hi < -60.0f;
+  const float half_way = ex(far ? 0.5f * (mo - m) : mo - m);
+  const float rest_to = mo > -INFINITY ? (far ? half_way * half_way : half_way) : 0.0f, top_to = top > -INFINITY ? ex(top - m) : 0.0f;
   const float scale = m < INFINITY ? factor : NAN, inv = scale / (so * rest_to + on * top_to);
   g.reference = mo;
   g.outside = so > 0.0f ? rest_to * inv - rest / so * scale : scale * 0.0f;

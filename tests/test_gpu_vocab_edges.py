@@ -101,3 +101,17 @@ def test_softmax_of_rows_that_rise_late(ctx, rows, vocab):
     ctx.check(rt.lib().rt_softmax_dev(ctx._h, z.ptr, 0, rows, vocab, vocab, 1.0, p.ptr, 0, vocab))
     _sync(ctx)
     _check_prob(p.read(), z, 1.0, "f32")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,vocab", [(160, 2100), (160, 12000), (2, 65536)])
+def test_gradients_far_below_the_list(ctx, rows, vocab, dtype):
+    """The student's mass lies on the list; outside of it probabilities down to 2^-126 of the largest are there."""
+    z = np.tile(_steps(vocab), (rows, 1))
+    z[:, -3] = 0.0
+    z[::2, 77] = z[1::2, vocab - 100] = 88.0
+    z = Rows(z, dtype)
+    index = np.array([[77, 5], [vocab - 100, 5]] * (rows // 2), np.int32)
+    t = np.log(np.array([[0.75, 0.25]] * rows))
+    got = _distill(ctx, z, index, t, 1.0, "renorm", None, "f32")
+    _check_distill(got, z, index, t, 1.0, "renorm", None, "f32")
