@@ -161,7 +161,7 @@ __global__ void __launch_bounds__(VD_THREADS) verify_draft_kernel(const T* P, si
     }
     total = __shfl_sync(0xffffffffu, up, 31);
     if (!(total > 0.0)) continue;
-    want = u < 0.0f ? 0.0 : (double)u * total;
+    want = u < 0.0f ? 0.0 : u < 1.0f ? (double)u * total : INFINITY;  // (from 1 on, and a NaN: no running sum exceeds it, however it was rounded)
     double in_front = __shfl_up_sync(0xffffffffu, up, 1);  // of the lane's two pieces
     if (lane == 0) in_front = 0.0;
     const unsigned over0 = __ballot_sync(0xffffffffu, m0 > 0.0 && in_front + m0 > want), over1 = __ballot_sync(0xffffffffu, m1 > 0.0 && up > want);

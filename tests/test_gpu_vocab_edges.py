@@ -115,3 +115,22 @@ def test_gradients_far_below_the_list(ctx, rows, vocab, dtype):
     t = np.log(np.array([[0.75, 0.25]] * rows))
     got = _distill(ctx, z, index, t, 1.0, "renorm", None, "f32")
     _check_distill(got, z, index, t, 1.0, "renorm", None, "f32")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_a_number_that_is_not_below_one_gives_the_last_index(ctx, dtype):
+    """However the running sums were rounded: masses whose sums are not exact, and next to nothing in the last place."""
+    rng = np.random.default_rng(0)
+    vocab, n = 16384, 300
+    p = np.zeros((n, vocab))
+    for r in range(n):
+        at = rng.integers(0, vocab - 1000, 60)
+        p[r, at] = rng.random(60)
+        p[r, at + 1] = rng.random(60) * 2.0**-33
+        p[r, vocab - 1 - r] = 1e-25
+        p[r, vocab - r:] = 0
+    P = Rows(p, dtype)
+    want = [int(np.nonzero(row)[0][-1]) for row in P.f64]
+    for u in (1.0, 2.0, np.inf, np.nan):
+        acc, token = _verify(ctx, P, None, [], [0] * (n + 1), [], [u] * n)
+        assert (acc == 0).all() and token.tolist() == want, u
