@@ -246,7 +246,10 @@ rt_status rt_top_logits_dev(rt_ctx* ctx, const void* logits_dev, int dtype, size
  * weight_dev [rows] (NULL: ones): a row of weight 0 gets zeros, whatever it holds.  loss_dev [rows] may be NULL, and so may
  * dlogits_dev ([rows x vocab], rows d_ld apart, of d_dtype; the logits' own place is allowed, any other overlap is not).
  * row_scale_dev (optional, [rows]): the gradients are written without the factor w / T, which goes there: the form that
- * rt_linear_backward_dev takes, in which f16 keeps its digits whatever the weights are. */
+ * rt_linear_backward_dev takes, in which f16 keeps its digits whatever the weights are.  f16 gradients below 2^-25 are 0 all
+ * the same, and outside of the list they all have one sign: over a large vocabulary much of their sum can be lost that way
+ * (a third of it, for 32 of 151936 entries and a student close to its teacher).  f32 and bf16 keep them, and so does
+ * rt_model_distill_backward, whose f16 rows are multiplied by 2^15. */
 rt_status rt_distill_dev(rt_ctx* ctx, const void* logits_dev, int dtype, size_t rows, size_t vocab, size_t ld,
                          float temperature, const int32_t* index_dev, const float* teacher_logp_dev, int k, int mode,
                          const float* weight_dev, float* loss_dev, void* dlogits_dev, int d_dtype, size_t d_ld,

@@ -1282,7 +1282,7 @@ static rt_status model_head(rt_model* m, int M, int n_targets, bool backward, fl
     }
     if (m->head.kind == rt_model::HEAD_DISTILL) {
       const DistillArgs a{rows, V, k, m->head.mode, m->head.temperature, m->list_index() + (size_t)c0 * k, m->list_logp() + (size_t)c0 * k,
-                          m->tw + c0, m->logp() + c0, m->dl16.p, RT_DT_F16, (size_t)V, m->sc_l.as<float>()};
+                          m->tw + c0, m->logp() + c0, m->dl16.p, RT_DT_F16, (size_t)V, m->sc_l.as<float>(), true};
       if (launch_distill_rows(c, a, R)) return c->fail(RT_ERR_CUDA, "distillation launch failed");
     } else if (launch_ce_rows(c, m->logits.as<float>(), R, V, m->ttok + c0, m->tw + c0, m->logp() + c0, m->hits(),
                               backward ? m->dl16.as<__half>() : nullptr, backward ? m->sc_l.as<float>() : nullptr,

@@ -92,7 +92,7 @@ rt_status rt_distill_dev(rt_ctx* c, const void* logits, int dtype, size_t rows, 
   }
   RT_CUDA(c, cudaSetDevice(c->device));
   const DistillArgs a{{logits, dtype, ld}, (int)vocab, k, mode, temperature, index, teacher_logp, weight, loss, dlogits,
-                      dlogits ? d_dtype : RT_DT_F32, d_ld, row_scale};
+                      dlogits ? d_dtype : RT_DT_F32, d_ld, row_scale, false};
   if (launch_distill_rows(c, a, rows)) return c->fail(RT_ERR_CUDA, "distillation launch failed");
   return RT_OK;
 }

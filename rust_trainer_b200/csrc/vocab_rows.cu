@@ -237,8 +237,13 @@ softmax_rows_kernel(const T* z, size_t ld, size_t rows, int vocab, ExpT ex, O* p
 // left (-1: the list has no mass that the student could learn from); by what its probabilities are divided, inverted; the largest logit.
 struct alignas(16) ListStat {
   double listed, by;  // (64 bits: what host lists call log-probabilities may be far from 0, all of them)
-  float rest, top, listed32, unused;
+  float rest, top, listed32, spread;  // spread: by what the row's gradients are multiplied, beside the factor w / T
 };
+// Gradients are at most the larger of 1 and the teacher's listed mass, most of those over a large vocabulary a millionth of it: times 2^15 f16 holds
+// the largest, and the small ones, which all have one sign outside of the list, do not round to 0 together.
+__device__ __forceinline__ float spread_of(float mass) {
+  return mass <= 1.0f ? 32768.0f : mass < INFINITY ? __uint_as_float((127 + 14 + 127 - (__float_as_uint(mass) >> 23)) << 23) : 1.0f;  // 2^(14 - exponent)
+}
 // a list of less mass than this has none
 constexpr double LEAST_MASS = 1e-300;
 // what a list leaves of a teacher's mass; a NaN stays
@@ -253,7 +258,7 @@ struct RowGradient {
   double by;
   bool idle;
 };
-template <int WARPS>
+template <int WARPS, bool SPREADS>
 __device__ __forceinline__ RowGradient row_gradient(const RowStat* stat, const ListStat* list, int size, bool idle, float factor, const ExpT& ex) {
   RowGradient g;
   float mo;
@@ -264,6 +269,7 @@ __device__ __forceinline__ RowGradient row_gradient(const RowStat* stat, const L
   const bool far = (mo - m) * ex.hi < -60.0f;
   const float half_way = ex(far ? 0.5f * (mo - m) : mo - m);
   const float rest_to = mo > -INFINITY ? (far ? half_way * half_way : half_way) : 0.0f, top_to = top > -INFINITY ? ex(top - m) : 0.0f;
+  if (SPREADS) factor *= list[0].spread;
   const float scale = m < INFINITY ? factor : NAN, inv = scale / (so * rest_to + on * top_to);
   g.reference = mo;
   g.outside = so > 0.0f ? rest_to * inv - rest / so * scale : scale * 0.0f;
@@ -294,9 +300,10 @@ __device__ __forceinline__ bool take_out(uint4* slots, int element) {
 template <class T, class O, int NT>
 __global__ void __maxnreg__(72)
 distill_rows_kernel(const T* z, size_t ld, size_t rows, int vocab, float t, ExpT ex, const int* index, const float* teacher, int k, int tail,
-                    const float* weight, float* loss, O* d, size_t d_ld, float* row_scale, int places, int* status) {
+                    const float* weight, float* loss, O* d, size_t d_ld, float* row_scale, int spread, int places, int* status) {
   using Ring = UnitRing<T, NT, ROW_STEP>;
   constexpr int WARPS = NT / 32, LIST_WARPS = RT_TOP_MAX / 32, VEC = Ring::VEC;
+  constexpr bool SPREADS = std::is_same<T, float>::value && std::is_same<O, __half>::value;  // what the model driver asks for; elsewhere `spread` is off
   extern __shared__ uint4 slots[];
   __shared__ RowBars b;
   __shared__ RowStat stats[4][VR_MAX_CLUSTER * WARPS];
@@ -332,7 +339,7 @@ distill_rows_kernel(const T* z, size_t ld, size_t rows, int vocab, float t, ExpT
       const float w = weight ? weight[r] : 1.0f, factor = row_scale ? 1.0f : w / t;
       ring.begin(z + r * ld);
       row_wait_turn(b.exchange, i, 2, status);
-      const RowGradient g = row_gradient<WARPS>(stats[i & 3], lists[i & 3], ring.size, w == 0.0f, factor, ex);
+      const RowGradient g = row_gradient<WARPS, SPREADS>(stats[i & 3], lists[i & 3], ring.size, w == 0.0f, factor, ex);
       row_wait_turn(b.summed, i, 1, status);
       // (rows that nothing is learnt from, whatever their logits are, have zeros)
       if (!g.idle) {
@@ -379,7 +386,8 @@ distill_rows_kernel(const T* z, size_t ld, size_t rows, int vocab, float t, ExpT
         }
       }
       if (d) {
-        const RowGradient g = row_gradient<WARPS>(stat, list, ring.size, w == 0.0f, row_scale ? 1.0f : w / t, ex);
+        if (row_scale && lane == 0 && ring.rank == 0) row_scale[r] = SPREADS ? w / t / list[0].spread : w / t;
+        const RowGradient g = row_gradient<WARPS, SPREADS>(stat, list, ring.size, w == 0.0f, row_scale ? 1.0f : w / t, ex);
         row_wait_turn(b.listed, i, 1, status);
         row_wait_turn(b.written, i, 1, status);
         for (int j = lane; j < k; j += 32) {
@@ -428,7 +436,6 @@ distill_rows_kernel(const T* z, size_t ld, size_t rows, int vocab, float t, ExpT
       const int next_entry = next_r < rows ? entry(next_r, &next_tl) : -1;
       if (i >= 2) row_wait_turn(b.exchange, i - 2, 2, status);  // not further ahead: the barriers tell two rows apart
       ring.begin(z + r * ld);
-      if (row_scale && me == 0 && ring.rank == 0) row_scale[r] = (weight ? weight[r] : 1.0f) / t;
       auto place_of = [&](int u, uint32_t* phase) {
         const int n = ring.place + u;
         *phase = ring.phase ^ (n < ring.places ? 0u : 1u);
@@ -504,11 +511,12 @@ distill_rows_kernel(const T* z, size_t ld, size_t rows, int vocab, float t, ExpT
         for (int j = 0; j < list_warps; ++j) mass += s_sums[j][0], cross += s_sums[j][1], on += s_sums[j][2];
         const float rest = tail ? (float)left_of(mass) : mass < LEAST_MASS ? -1.0f : 0.0f;
         const double by = tail ? 1.0 : 1.0 / mass;
+        const float times = SPREADS && spread ? spread_of(tail ? (float)mass : 1.0f) : 1.0f;
         const uint64_t* bar = b.exchange + (i & 3);
         if (lane < ring.size) {
           const uint32_t to = mapa_u32(smem_u32(&lists[i & 3][ring.rank]), lane), its_bar = mapa_u32(smem_u32(bar), lane);
           send(to, its_bar, (uint32_t)__double2loint(on), (uint32_t)__double2hiint(on), (uint32_t)__double2loint(by), (uint32_t)__double2hiint(by));
-          send(to + 16, its_bar, __float_as_uint(rest), __float_as_uint(top), __float_as_uint((float)on), 0u);
+          send(to + 16, its_bar, __float_as_uint(rest), __float_as_uint(top), __float_as_uint((float)on), __float_as_uint(times));
         }
         if (finds_loss && lane == 0)
           send(mapa_u32(smem_u32(&losses[i & 3]), 0), mapa_u32(smem_u32(bar), 0), (uint32_t)__double2loint(mass), (uint32_t)__double2hiint(mass),
@@ -578,7 +586,7 @@ int launch_distill_rows(rt_ctx* c, const DistillArgs& a, size_t rows) {
         using O = std::remove_pointer_t<decltype(ot)>;
         return launch_clusters(c, distill_rows_kernel<T, O, decltype(threads)::value>, true, rows, all_threads, shape.cluster, shape.smem, (const T*)a.z.p,
                                a.z.ld, rows, a.vocab, a.temperature, exp_t(a.temperature), a.index, a.teacher, a.k, a.mode == RT_DISTILL_TAIL, a.weight,
-                               a.loss, (O*)a.d, a.d_ld, a.row_scale, shape.places, c->status_dev);
+                               a.loss, (O*)a.d, a.d_ld, a.row_scale, a.spread, shape.places, c->status_dev);
       });
     });
   });

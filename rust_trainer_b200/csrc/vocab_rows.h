@@ -28,6 +28,7 @@ struct DistillArgs {
   int d_dtype;
   size_t d_ld;
   float* row_scale;       // [rows] or null: the factor w / T, which d then does not hold
+  bool spread;            // f32 rows, f16 gradients with row_scale: these times a power of two, 2^15 as a rule, which row_scale takes back
 };
 int launch_distill_rows(rt_ctx* c, const DistillArgs& a, size_t rows);
 
