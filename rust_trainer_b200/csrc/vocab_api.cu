@@ -11,12 +11,19 @@ bool bad_dtype(int dtype) { return dtype != RT_DT_F32 && dtype != RT_DT_BF16 && 
 bool unaligned(const void* p, size_t to) { return (uintptr_t)p % to != 0; }
 bool bad_temperature(float t) { return !(t >= 1e-4f && t <= 1e4f); }
 
-// Whether the rows of `in` and `out` share bytes, other than by lying in the same place element by element.
+// Whether the rows of `in` and `out` share bytes, other than by lying in the same place element by element.  Rows of one pitch may lie between one another;
+// where the pitches differ, everything from the first row's start to the last one's end counts.
 bool overlap(const void* in, size_t in_ld, int in_dtype, const void* out, size_t out_ld, int out_dtype, size_t rows, size_t vocab) {
   if (in == out && in_dtype == out_dtype && (in_ld == out_ld || rows == 1)) return false;
   const uintptr_t a = (uintptr_t)in, b = (uintptr_t)out;
-  const size_t na = ((rows - 1) * in_ld + vocab) * dtype_bytes(in_dtype), nb = ((rows - 1) * out_ld + vocab) * dtype_bytes(out_dtype);
-  return a < b + nb && b < a + na;
+  const size_t pa = in_ld * dtype_bytes(in_dtype), pb = out_ld * dtype_bytes(out_dtype), wa = vocab * dtype_bytes(in_dtype), wb = vocab * dtype_bytes(out_dtype);
+  const size_t na = (rows - 1) * pa + wa, nb = (rows - 1) * pb + wb;
+  if (!(a < b + nb && b < a + na)) return false;
+  if (pa != pb) return true;
+  // the later one's first row begins `at` bytes behind the other's row above it, and reaches into that row or the next one, if there is one
+  const bool in_first = a <= b;
+  const size_t apart = in_first ? b - a : a - b, at = apart % pa, w_first = in_first ? wa : wb, w_later = in_first ? wb : wa;
+  return at < w_first || (at + w_later > pa && apart / pa + 1 < rows);
 }
 
 rt_status check_rows(rt_ctx* c, const void* p, int dtype, size_t rows, size_t vocab, size_t ld) {

@@ -134,3 +134,45 @@ def test_a_number_that_is_not_below_one_gives_the_last_index(ctx, dtype):
     for u in (1.0, 2.0, np.inf, np.nan):
         acc, token = _verify(ctx, P, None, [], [0] * (n + 1), [], [u] * n)
         assert (acc == 0).all() and token.tolist() == want, u
+
+
+def test_results_between_the_rows(ctx):
+    """Rows and results may share an allocation as long as they share no bytes: halves of the same rows, or rows in turn."""
+    import torch
+
+    rng = np.random.default_rng(2)
+    rows, vocab = 4, 1000
+    v = _logits(rng, rows, vocab)
+    z = Rows(v, "f32")
+    index, t = _lists(rng, z, 9, 1.0)
+    i, tl = _dev(index, torch.int32), _dev(t, torch.float32)
+    L = rt.lib()
+    store = torch.empty(rows * 2016 + 2016, device="cuda")
+    left, right = store[:rows * 2016].view(rows, 2016), store[1008:1008 + rows * 2016].view(rows, 2016)
+
+    def fresh():
+        store.fill_(float("nan"))
+        left[:, :vocab] = torch.as_tensor(v).cuda()
+        _before()
+
+    fresh()
+    ctx.check(L.rt_softmax_dev(ctx._h, left.data_ptr(), 0, rows, vocab, 2016, 1.0, right.data_ptr(), 0, 2016))
+    _sync(ctx)
+    _check_prob(right[:, :vocab].double().cpu().numpy(), z, 1.0, "f32")
+    assert np.array_equal(left[:, :vocab].cpu().numpy(), v) and bool(torch.isnan(left[:, vocab:1008]).all())
+    fresh()
+    loss = _empty((rows,))
+    ctx.check(L.rt_distill_dev(ctx._h, left.data_ptr(), 0, rows, vocab, 2016, 1.0, i.data_ptr(), tl.data_ptr(), 9, 1, None, loss.data_ptr(),
+                               right.data_ptr(), 0, 2016, None))
+    _sync(ctx)
+    _check_distill((loss.cpu().numpy().astype(np.float64), right[:, :vocab].double().cpu().numpy(), None, None), z, index, t, 1.0, "tail", None, "f32")
+    # one element shared, in front or behind, is one too many
+    b = store.data_ptr()
+    for at in (vocab - 1, 2016 - vocab + 1):
+        assert L.rt_softmax_dev(ctx._h, b, 0, rows, vocab, 2016, 1.0, b + 4 * at, 0, 2016) == 7
+        assert L.rt_softmax_dev(ctx._h, b + 4 * at, 0, rows, vocab, 2016, 1.0, b, 0, 2016) == 7
+    # 16-bit results of the same pitch, behind the row or one element too early
+    assert L.rt_softmax_dev(ctx._h, b, 0, rows, vocab, 2016, 1.0, b + 4 * vocab, 2, 4032) == 0
+    assert L.rt_softmax_dev(ctx._h, b, 0, rows, vocab, 2016, 1.0, b + 4 * vocab - 2, 2, 4032) == 7
+    assert L.rt_softmax_dev(ctx._h, b, 0, rows, vocab, 2016, 1.0, b + 4 * vocab, 2, 4030) == 7  # another pitch
+    _sync(ctx)
