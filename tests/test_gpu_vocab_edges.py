@@ -176,3 +176,78 @@ def test_results_between_the_rows(ctx):
     assert L.rt_softmax_dev(ctx._h, b, 0, rows, vocab, 2016, 1.0, b + 4 * vocab - 2, 2, 4032) == 7
     assert L.rt_softmax_dev(ctx._h, b, 0, rows, vocab, 2016, 1.0, b + 4 * vocab, 2, 4030) == 7  # another pitch
     _sync(ctx)
+
+
+@pytest.mark.parametrize("mode", ["renorm", "tail"])
+@pytest.mark.parametrize("vocab", [500, 50021])
+def test_rows_beside_one_with_an_index_outside(ctx, vocab, mode):
+    """What such a call leaves: the other rows' losses and gradients."""
+    import torch
+
+    rng = np.random.default_rng(13)
+    rows, k = 7, 5
+    z = Rows(_logits(rng, rows, vocab), "f32")
+    index, t = _lists(rng, z, k, 1.0)
+    tl = _dev(t, torch.float32)
+    for bad in (vocab, -2, 2**31 - 1, -2**31):
+        wrong = index.copy()
+        wrong[3, 2] = bad
+        i, loss, d = _dev(wrong, torch.int32), _empty((rows,)), Rows(np.full((rows, vocab), np.nan), "f32")
+        _before()
+        ctx.check(rt.lib().rt_distill_dev(ctx._h, z.ptr, 0, rows, vocab, vocab, 1.0, i.data_ptr(), tl.data_ptr(), k, ops.DISTILL_MODES[mode], None,
+                                          loss.data_ptr(), d.ptr, 0, vocab, None))
+        with pytest.raises(rt.RtError) as e:
+            _sync(ctx)
+        assert e.value.status == 6
+        good = [r for r in range(rows) if r != 3]
+        some = Rows(z.f64[good], "f32")
+        _check_distill((loss.cpu().numpy().astype(np.float64)[good], d.read()[good], None, None), some, index[good], t[good], 1.0, mode, None, "f32")
+        assert d.others_untouched()
+
+
+@pytest.mark.parametrize("vocab", [300, 50021])
+def test_sequences_beside_one_that_does_not_fit(ctx, vocab):
+    """Such a sequence stands for nothing (0, -1); the others are what they are."""
+    import torch
+
+    rng = np.random.default_rng(3)
+    off, p, q, tok, ua, us = _drafts(rng, (2, 3, 2, 1), vocab)
+    P, Q = Rows(p, "f32"), Rows(q, "f32")
+    a, s = _dev(ua, torch.float32), _dev(us, torch.float32)
+    for change, bad in ((lambda t, o: t.__setitem__(3, vocab), [1]), (lambda t, o: t.__setitem__(4, -1), [1]), (lambda t, o: t.__setitem__(0, 2**31 - 1), [0]),
+                        (lambda t, o: o.__setitem__(1, 6), [0, 1]), (lambda t, o: o.__setitem__(2, 9), [1, 2]), (lambda t, o: o.__setitem__(0, 1), [0]),
+                        (lambda t, o: o.__setitem__(4, 7), [3]), (lambda t, o: o.__setitem__(1, -3), [0, 1]), (lambda t, o: o.__setitem__(4, 9), [3])):
+        t, o = np.asarray(tok, np.int32).copy(), np.asarray(off, np.int32).copy()
+        change(t, o)
+        tk, of, acc, token = _dev(t), _dev(o), _empty((4,), torch.int32), _empty((4,), torch.int32)
+        _before()
+        ctx.check(rt.lib().rt_verify_draft_dev(ctx._h, P.ptr, vocab, Q.ptr, vocab, 0, vocab, tk.data_ptr(), of.data_ptr(), 4, len(tok), a.data_ptr(),
+                                               s.data_ptr(), acc.data_ptr(), token.data_ptr()))
+        with pytest.raises(rt.RtError) as e:
+            _sync(ctx)
+        assert e.value.status == 6
+        acc, token = acc.cpu().numpy(), token.cpu().numpy()
+        # a sequence whose offsets are in order among themselves is taken as they say; only those that are as they were have a known answer
+        for i in range(4):
+            if i in bad and (o[i] < 0 or o[i + 1] < o[i] or o[i + 1] > len(tok) or (i == 0 and o[0]) or (i == 3 and o[4] != len(tok)) or
+                             not ((t[o[i]:o[i + 1]] >= 0) & (t[o[i]:o[i + 1]] < vocab)).all()):
+                assert (int(acc[i]), int(token[i])) == (0, -1), i
+            elif i not in bad:
+                lo, hi = off[i], off[i + 1]
+                assert (int(acc[i]), int(token[i])) == R.verify(P.f64[lo + i:hi + i + 1], Q.f64[lo:hi], tok[lo:hi], ua[lo:hi], us[i]), i
+
+
+@pytest.mark.parametrize("temperature", [1e-4, 1e4])
+@pytest.mark.parametrize("rows,vocab,dtype", [(5, 37, "f32"), (3, 50021, "f32"), (3, 50021, "bf16"), (300, 3001, "f16"), (300, 3001, "f32")])
+def test_the_ends_of_the_temperature(ctx, rows, vocab, dtype, temperature):
+    rng = np.random.default_rng(vocab)
+    z = Rows(_logits(rng, rows, vocab), dtype, vocab + 3, 1)
+    for k in (1, 30):
+        _check_top(_top(ctx, z, k, temperature), z, k, temperature)
+    some = min(rows, 12)
+    index, t = _lists(rng, z, 12, temperature, 0.5)
+    for mode in ("renorm", "tail"):
+        ls, d, f, _ = _distill(ctx, z, index, t, temperature, mode, None, "f32")
+        z.rows = some
+        _check_distill((ls, d, f, None), z, index, t, temperature, mode, None, "f32")
+        z.rows = rows
