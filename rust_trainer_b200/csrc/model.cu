@@ -1728,7 +1728,9 @@ rt_status rt_model_verify_draft(rt_model* m, rt_model* draft, const int32_t* tok
     x->staged_targets = (int)pos.size();
     x->staged_has_weights = false;
     const HeadScope scope(x, rt_model::HEAD_NONE, 1.f, 0, 0, 0);
-    RT_TRY(run_staged(x, false, nullptr));
+    const rt_status st = run_staged(x, false, nullptr);
+    x->staged_tokens = 0;  // no batch to be scored, however the call goes on
+    if (st) return st;
   }
   // one block each way: tokens, random numbers, a chunk's offsets (from 0 on) behind one another; accepted, token
   std::vector<int32_t> block(tok);
@@ -1765,8 +1767,6 @@ rt_status rt_model_verify_draft(rt_model* m, rt_model* draft, const int32_t* tok
                        dev + o_res + n_seq + s0};
     if (launch_verify_draft(c, a)) return c->fail(RT_ERR_CUDA, "verification launch failed");
   }
-  for (rt_model* x : {m, draft})
-    if (x) x->staged_tokens = 0;
   RT_CUDA(c, cudaMemcpyAsync(accepted_out, dev + o_res, (size_t)n_seq * 4, cudaMemcpyDeviceToHost, c->stream));
   RT_CUDA(c, cudaMemcpyAsync(token_out, dev + o_res + n_seq, (size_t)n_seq * 4, cudaMemcpyDeviceToHost, c->stream));
   return c->check_device_status("rt_model_verify_draft");

@@ -79,3 +79,19 @@ def test_lists_of_more_than_all_mass(ctx, preset):
         got = (gradient(np.log(mass), "tail") - one) * 2 / (mass - 1)
         assert rel_l2(got, want) < 1e-2 and cosine(got, want) > 0.999, mass
     m.close()
+
+
+def test_a_verification_that_fails_leaves_no_batch_behind(ctx):
+    """The drafting model refuses its pass (it has no weights yet) when the target's has run."""
+    spec, m = _model(ctx, head_rows=16)
+    d = rt.Model.__new__(rt.Model)
+    with pytest.raises(rt.RtError):
+        d.__init__(ctx, spec.config(), {}, head_rows=16)
+    seqs = _seqs(spec, [20])
+    with pytest.raises(rt.RtError) as e:
+        m.verify_draft(seqs, [15], [0.5] * 5, [0.5], draft=d)
+    assert "finalize" in str(e.value)
+    assert rt.lib().rt_model_run_staged(m._h, 0) == 7
+    assert np.isfinite(m.score(seqs, np.array([3], np.int32), [1])[0]).all()
+    m.close()
+    d.close()
