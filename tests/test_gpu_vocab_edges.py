@@ -251,3 +251,14 @@ def test_the_ends_of_the_temperature(ctx, rows, vocab, dtype, temperature):
         z.rows = some
         _check_distill((ls, d, f, None), z, index, t, temperature, mode, None, "f32")
         z.rows = rows
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("vocab", [4097, 4400, 8692, 12800, 16884, 20600])
+def test_top_logits_of_rows_whose_last_unit_is_short(ctx, vocab, dtype):
+    """The last unit of a row holds elements for a few warps only: such rows find their bound in the CTAs that have more."""
+    rng = np.random.default_rng(vocab)
+    for rows in (1, 16, 120):
+        z = Rows(_logits(rng, rows, vocab), dtype, vocab + 3, 1)
+        for k in (8, 64, 200):
+            _check_top(_top(ctx, z, k, 1.0), z, k, 1.0)
