@@ -1648,7 +1648,9 @@ rt_status rt_model_top_logits(rt_model* m, const int32_t* tokens, const int32_t*
   m->staged_targets = n_targets;
   m->staged_has_weights = false;
   const HeadScope scope(m, rt_model::HEAD_TOP, temperature, k, 0, n_targets);
-  RT_TRY(run_staged(m, false, nullptr));
+  const rt_status st = run_staged(m, false, nullptr);
+  m->staged_tokens = 0;  // its targets' tokens are none: not to be run as a scoring batch
+  if (st) return st;
   RT_CUDA(c, cudaMemcpyAsync(index_out, m->list_index(), n * k * 4, cudaMemcpyDeviceToHost, c->stream));
   RT_CUDA(c, cudaMemcpyAsync(logp_out, m->list_logp(), n * k * 4, cudaMemcpyDeviceToHost, c->stream));
   if (lse_out) RT_CUDA(c, cudaMemcpyAsync(lse_out, m->list_logp() + n * k, n * 4, cudaMemcpyDeviceToHost, c->stream));

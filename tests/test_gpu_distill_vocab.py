@@ -95,3 +95,12 @@ def test_a_verification_that_fails_leaves_no_batch_behind(ctx):
     assert np.isfinite(m.score(seqs, np.array([3], np.int32), [1])[0]).all()
     m.close()
     d.close()
+
+
+def test_no_scoring_batch_is_staged_behind_a_teachers_pass(ctx):
+    spec, m = _model(ctx)
+    seqs, pos = _seqs(spec, [20, 9]), np.array([3, 8, 25], np.int32)
+    m.top_logits(seqs, pos, 4)
+    assert rt.lib().rt_model_run_staged(m._h, 0) == 7
+    assert np.isfinite(m.score(seqs, pos, [1, 2, 3])[0]).all()
+    m.close()
