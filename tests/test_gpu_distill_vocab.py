@@ -104,3 +104,23 @@ def test_no_scoring_batch_is_staged_behind_a_teachers_pass(ctx):
     assert rt.lib().rt_model_run_staged(m._h, 0) == 7
     assert np.isfinite(m.score(seqs, pos, [1, 2, 3])[0]).all()
     m.close()
+
+
+@pytest.mark.parametrize("mode", ["renorm", "tail"])
+def test_distillation_in_chunks_of_the_head(ctx, mode):
+    """Five targets through a head of two rows at a time: the losses of one chunk, and its gradients."""
+    spec, m = _model(ctx)
+    _, small = _model(ctx, head_rows=2)
+    seqs, pos = _seqs(spec, [30, 12]), np.array([3, 20, 29, 31, 40], np.int32)
+    w = np.array([0.2, 0.1, 0.3, 0.0, 0.4], np.float32)
+    rng = np.random.default_rng(7)
+    index = rng.integers(0, spec.vocab, (5, 9)).astype(np.int32)
+    t = np.log(rng.dirichlet(np.ones(10), 5)[:, :9])
+    out = []
+    for x in (m, small):
+        x.zero_grad()
+        out.append((x.distill_backward(seqs, pos, index, t, w, 1.5, mode), _gpu_flat(x, "ga", "gb")))
+    assert np.abs(out[0][0] - out[1][0]).max() <= 256 * U
+    assert rel_l2(out[1][1], out[0][1]) < 1e-2 and cosine(out[1][1], out[0][1]) > 0.999
+    m.close()
+    small.close()
