@@ -219,12 +219,13 @@ rt_status rt_op_cross_entropy(rt_ctx* ctx, const float* logits_host, size_t rows
  *   - a probability below 2^-126 of the row's largest may come out as 0;
  *   - among equal values (the two zeros are equal) the lowest index comes first.
  * Rows are `ld` elements apart (ld >= vocab; what lies behind the vocabulary is neither read nor written),
- * their elements RT_DT_F32, RT_DT_BF16 or RT_DT_F16; any element-aligned address is taken.  Results may lie in the logits' own
- * place where that is said, or between the rows if both have as many bytes from row to row; they may share no byte otherwise.  Sums over a row are
- * held in 32 bits within a warp, and from there in 64 for log-sum-exps and losses, in 32 for probabilities and
- * gradients.  The device forms only launch on the ctx stream: they allocate no device memory, share no workspace
- * and may be captured; what a kernel finds wrong (an index out of range) is reported by the next
- * rt_ctx_synchronize, like a wait that ran out.  The host forms take f32 rows. */
+ * their elements RT_DT_F32, RT_DT_BF16 or RT_DT_F16; any element-aligned address is taken.  Results may lie in the
+ * logits' own place where that is said, or between the rows if both have as many bytes from row to row; they may share
+ * no byte otherwise.  Sums over a row are held in 32 bits within a warp (losses: within two), and from there in 64 for
+ * log-sum-exps and losses, in 32 for probabilities and gradients; a list's own sums in 64.  The device forms only launch
+ * on the ctx stream: they allocate no device memory, share no workspace and may be captured; what a kernel finds wrong
+ * (an index out of range) is reported by the next rt_ctx_synchronize, like a wait that ran out, and spoils its own row
+ * or sequence only.  The host forms take f32 rows. */
 #define RT_TOP_MAX 256      /* entries of a teacher's list, at most */
 #define RT_VOCAB_MAX 393216 /* elements of a row, at most */
 /* What becomes of the probability that a teacher's list leaves out: the list is normalised to one, or the rest is one

@@ -6,8 +6,8 @@
 // counting the larger ones.  Only where elements kept or left are too many (values that tie, masked rows, rows in ascending order) the row
 // is read again, for a better bound by bisection over values and indices.
 //
-// Measured, against the bytes at the rate of a copy: 64 of 1024 x 151936 f32 140 us (floor 96, 4.5 TB/s), 32 of 4096 x 128256 bf16 365 us (163), 8 of
-// one row of 151936 f32 13 us.  What bounds it is instructions and their latency: 46 % of the issue slots are taken, an exponential, a comparison
+// Measured, against the bytes at the rate of a copy: 64 of 1024 x 151936 f32 138 us (floor 96, 4.5 TB/s), 32 of 4096 x 128256 bf16 358 us (163), 8 of
+// one row of 151936 f32 12 to 13 us.  What bounds it is instructions and their latency: 46 % of the issue slots are taken, an exponential, a comparison
 // and a share of the largest for each element, 28 % of the special-function unit; three CTAs on an SM fill each other's waits at row ends
 // (sorting of the sample, exchange, ranks: some 8 us a row).  One row alone is launch, a copy's latency and those.
 #include "vocab_rows.cuh"

@@ -2,10 +2,10 @@
 // then each warp sums a contiguous piece of the row that the next token is drawn from, the warps' sums go to all CTAs, and the warp whose
 // piece holds the token looks for it there, in the eighth of the piece that its own sums point to.  The row is read once.
 //
-// Measured: one sequence with four drafts over 151936 f32 12 to 15 us, 96 with up to eight over 128256 bf16 25 us (floor 5.7), 32 with up to three
-// certain ones over 151936 f32 21 to 24 us (3).  What bounds it: dependent loads (offsets, tokens, their probabilities, the row, the piece once
-// more), and for many sequences the arithmetic of exact sums, 57 % of all issue slots.  512 threads took 42 us for the 32; sums of two floats on packed
-// pairs took more registers and the same time.
+// Measured: one sequence with four drafts over 151936 f32 12 to 13 us, 96 with up to eight over 128256 bf16 26.5 us (floor 5.7), 32 with up to three
+// certain ones over 151936 f32 17 to 22 us (3).  What bounds it: dependent loads (offsets, tokens, their probabilities, the row, the piece once
+// more), and for many sequences the arithmetic of exact sums: 62 % of the issue slots of SMs that work, 42 % of all.  512 threads took 42 us for the
+// 32; sums of two floats on packed pairs took more registers and the same time.
 #include "vocab_rows.cuh"
 
 namespace rt {
@@ -228,10 +228,11 @@ __global__ void __launch_bounds__(VD_THREADS) verify_draft_kernel(const T* P, si
 }
 
 int launch_verify_draft(rt_ctx* c, const VerifyArgs& a) {
-  // As many CTAs a sequence as run at once for all of them, three on an SM: a second wave costs more than a longer row.  In us, by the cluster's size:
-  //   1 of 30000 f32   1: 20.2, 2: 14.3, 4 and 8: 12.3       1 of 6000 f32: the same with any
-  //   64 of 30000 f32   1: 32.8, 2: 22.5, 4: 17.7, 8: 24.0    96 of 128256 bf16   2: 41.0, 4: 30.7, 8: 34.6
-  //   200 of 128256 bf16   1: 74, 2: 52, 4: 53, 8: 58         1000 of 9000 bf16   1: 39, 2: 61, 8: 202
+  // As many CTAs a sequence as run at once for all of them, three on an SM: a second wave costs more than a longer row.  In us, one call after the
+  // other, by the cluster's size (drafts with probabilities):
+  //   1 of 30000 f32   1: 15.9, 2: 11.0, 4 and 8: 8.3        1 of 151936 f32   1: 51.8, 2: 30.3, 4: 17.8, 8: 13.4       1 of 6000 f32: the same with any
+  //   64 of 30000 f32   1: 28.8, 2: 18.5, 4: 12.9, 8: 19.9    96 of 128256 bf16   1: 55.7, 2: 34.1, 4: 25.0, 8: 27.0
+  //   200 of 128256 bf16   1: 67.1, 2: 46.7, 4: 45.9, 8: 52.9    1000 of 9000 bf16   1: 35.3, 2: 58.5, 4: 106, 8: 202
   int size = 1;
   while (a.vocab >= 8192 && size < VR_MAX_CLUSTER && (size_t)a.n_seq * size * 2 <= 3 * (size_t)c->num_sms) size *= 2;
   return with_dtype(a.p.dtype, [&](auto* t) {

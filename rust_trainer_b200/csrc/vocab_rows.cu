@@ -2,12 +2,12 @@
 // gone round.  In each CTA some warps sum row n + 1 while others write row n and the next ones are copied, so that memory is busy while sums
 // are found and go round, and a warp or a few make each row's list ready and find its loss.
 //
-// Measured, against the bytes at the rate of a copy: softmax of 1536 x 128256 bf16 into f32 207 us (floor 183, 5.7 TB/s); gradients of
-// 1024 x 151936 f32 in f16 from 64 entries 219 us (144), of 2048 x 128256 bf16 from 32 250 us (162); losses alone of 777 x 50021 f16
+// Measured, against the bytes at the rate of a copy: softmax of 1536 x 128256 bf16 into f32 219 to 226 us (floor 183, 5.2 to 5.4 TB/s); gradients of
+// 1024 x 151936 f32 in f16 from 64 entries 215 us (144), of 2048 x 128256 bf16 from 32 244 to 248 us (162); losses alone of 777 x 50021 f16
 // 37 us (12).  (All warps at one row after the other, with the same copies ahead: 285, 264, 283 and 37 us.)  What bounds distillation is the
 // chain of a row: its last unit's copy (some 4500 of the f32 row's 17300 cycles over two rows), the sums (4700), the exchange and the coefficients
 // (3200), the writing (4000), and two rows are all that a cluster's shared memory holds.  A wait on a barrier costs 100 to 200 cycles in
-// these loops: whoever is told of a whole row does not wait for its units (240 -> 219 us).  Tried without gain, in us for the f32 rows: units in pairs
+// these loops: whoever is told of a whole row does not wait for its units (219 -> 215 us, 269 -> 244).  Tried without gain, in us for the f32 rows: units in pairs
 // (286), lists that are taken out unit by unit so that sums begin behind the copy (248), entries that each wait for their own unit (233), two CTAs
 // on an SM with half of the row each (420 and more), clusters that start one after the other, the factor in the exponent for 16-bit results (the same).
 //
@@ -125,7 +125,8 @@ __device__ __forceinline__ void sum_rows(UnitRing<T, NT, ROW_STEP>& ring, const 
 // One row's results into `out`, by the warps that write: (16-bit rows) e f, e the exponentials relative to the row's reference, or (32-bit rows, whose
 // exponentials are there relative to the thread's reference `mine`) those times what that makes f.  Gives the units back.
 // PACED: with a wait for each unit, which the warps that sum have seen full already.  Where memory binds it spreads the stores: softmax of 1536 x
-// 128256 bf16 rows, one call after the other, takes 211 to 221 us with it and 229 without; distillation of 1024 x 151936 f32 rows 240 and 219.
+// 128256 bf16 rows, one call after the other, takes 220 us with it and 224 without; distillation of 1024 x 151936 f32 rows 219 and 215, of
+// 2048 x 128256 bf16 rows 269 and 244.
 template <bool PACED, class O, class T, int NT>
 __device__ __forceinline__ void write_row(UnitRing<T, NT, ROW_STEP>& ring, O* out, float mine, float reference, float f, const ExpT& ex) {
   using Ring = UnitRing<T, NT, ROW_STEP>;
