@@ -245,8 +245,9 @@ rt_status rt_top_logits_dev(rt_ctx* ctx, const void* logits_dev, int dtype, size
  *   TAIL:   q_j = exp(t_j), r = max(0, 1 - sum q), R = the student's mass outside the list;
  *           loss = w (sum q_j (t_j - s_{i_j}) + r (log r - log R));
  *           dz_v = (w / T) (p_v - q_v) inside the list, (w / T) p_v (1 - r / R) outside
- * weight_dev [rows] (NULL: ones): a row of weight 0 gets zeros, whatever it holds.  loss_dev [rows] may be NULL, and so may
- * dlogits_dev ([rows x vocab], rows d_ld apart, of d_dtype; the logits' own place is allowed, any other overlap is not).
+ * weight_dev [rows] (NULL: ones): a row of weight 0 gets zeros, whatever its logits are (its indices are checked all the
+ * same).  loss_dev [rows] may be NULL, and so may dlogits_dev ([rows x vocab], rows d_ld apart, of d_dtype; the logits' own
+ * place is allowed, any other overlap is not).
  * row_scale_dev (optional, [rows]): the gradients are written without the factor w / T, which goes there: the form that
  * rt_linear_backward_dev takes, in which f16 keeps its digits whatever the weights are.  f16 gradients below 2^-25 are 0 all
  * the same, and outside of the list they all have one sign: over a large vocabulary much of their sum can be lost that way

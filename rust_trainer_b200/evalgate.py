@@ -67,7 +67,7 @@ def greedy_prefix_batch(model, examples):
 def accepted_prefix(model, examples, rng, temperature: float = 1.0, draft=None):
     """The sampling counterpart of greedy_prefix_batch: per (tokens, answer_start) example, how long a prefix of the answer the
     model lets stand as drafts of `draft` (None: as drafts without probabilities), the answer's length, and the token that it
-    puts behind that prefix.  `rng` (a NumPy generator) gives the random numbers.  No counterpart in the reference."""
+    puts behind that prefix.  An answer is shorter than the models' head_rows, or the call is refused.  `rng` (a NumPy generator) gives the random numbers.  No counterpart in the reference."""
     exs = [(np.asarray(t, dtype=np.int32), max(int(a), 1)) for t, a in examples]
     exs = [(t, min(a, t.size)) for t, a in exs]
     if not exs:
